@@ -195,6 +195,66 @@ int tf_composite_bwd(const float* alpha, const int64_t* ray_indices, const float
                      int64_t n_rays, int32_t k, float* g_alpha, float* g_values, tf_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Packed sequences: tables of a ragged batch, and the gated linear recurrence that runs over it.
+ * The compositing above is one instance of it (a scalar gate per sample, the end state only; nerfacc call sites
+ * network/shapeRenderer.py:1166-1206); here a state of any width is kept at every row, and may begin at h0.
+ *
+ * tf_segment_tables: from lengths[n_segments] (values below 0 count as 0, above n_rows as n_rows)
+ *   offsets[n_segments + 1] = exclusive sums, cut at n_rows;  index[i] = the segment of row i (ray_indices);
+ *   position[i] = i - offsets[index[i]];  bit i % 64 of starts[i / 64] = row i is a segment's first ((n_rows + 63) / 64 words).
+ *   Rows behind the last segment have index and position -1 and no start bit.  index, position, starts may be NULL.
+ *   block_rows > 0: the rows of segment s live in blocks of block_rows rows of a shared store; its c-th block is
+ *   block_table[s, c] = free_blocks[sum_{q<s} ceil(lengths[q] / block_rows) + c], -1 behind its last block or the list's end;
+ *   slots[i] = block * block_rows + position % block_rows, -1 where there is no block or it lies behind max_blocks.
+ *   workspace: tf_segment_workspace_words(n_segments, block_rows) int64 words.
+ * tf_segment_from_index: offsets and starts from a sorted index[n_rows] (rows with an index outside [0, n_segments) are no segment's:
+ *   they stand in front of offsets[0] or from offsets[n_segments] on).
+ * ------------------------------------------------------------------------------------------ */
+size_t tf_segment_workspace_words(int64_t n_segments, int64_t block_rows);
+int tf_segment_tables(const int64_t* lengths, int64_t n_segments, int64_t n_rows, int64_t* offsets, int64_t* index, int64_t* position,
+                      uint64_t* starts, int64_t block_rows, const int32_t* free_blocks, int64_t n_free, int64_t max_blocks,
+                      int32_t* block_table, int64_t* slots, int64_t* workspace, size_t workspace_words, tf_stream_t stream);
+int tf_segment_from_index(const int64_t* index, int64_t n_rows, int64_t n_segments, int64_t* offsets, uint64_t* starts, tf_stream_t stream);
+
+typedef enum TfType { TF_TYPE_F32 = 0, TF_TYPE_F16 = 1, TF_TYPE_BF16 = 2 } TfType;
+typedef enum TfGateForm {
+  TF_GATE_DECAY = 0, /* h = g h + x */
+  TF_GATE_LOG = 1,   /* h = exp(g) h + x */
+  TF_GATE_ALPHA = 2  /* h = (1 - g) h + g x: compositing, leaky averages */
+} TfGateForm;
+
+/* x [n_rows, channels] and gate [n_rows, gates] with row strides in elements; one gate serves channels / gates consecutive channels.
+ * x is fp32, fp16 or bf16, the gate of the same type or fp32; states are fp32, y and the gradients are rounded once to their inputs' types. */
+typedef struct TfGatedScan {
+  int64_t n_rows, n_segments;
+  int64_t ld_x, ld_gate;
+  int32_t channels, gates;
+  int32_t x_type, gate_type; /* TfType */
+  int32_t form;              /* TfGateForm */
+  int32_t reverse;           /* 1: every segment runs from its last row to its first */
+  int32_t zero_rest;         /* rows of the results that are no segment's: 0 left as they were, 1 set to zero */
+} TfGatedScan;
+
+/* y [n_rows, channels] (x's type) = h of every row that is a segment's; final [n_segments, channels] or NULL:
+ * the state after the segment's last step, h0 (or 0) where it has no rows; h0 [n_segments, channels] or NULL.
+ * offsets / index / starts: of tf_segment_tables or tf_segment_from_index (index is read with h0 or final alone).  carry: NULL, or
+ * tf_gated_scan_carry_floats(d) floats that the backward pass needs.
+ * tf_gated_scan_bwd: gy [n_rows, channels] (x's type) and gfinal [n_segments, channels], either NULL; dgate [n_rows, gates], dx [n_rows, channels],
+ * dh0 [n_segments, channels], each NULL where it is not wanted.  No atomics on results: they repeat bit by bit. */
+size_t tf_gated_scan_carry_floats(const TfGatedScan* d);
+size_t tf_gated_scan_workspace_floats(const TfGatedScan* d, int32_t backward);
+int tf_gated_scan_fwd(const TfGatedScan* d, const void* gate, const void* x, const int64_t* offsets, const int64_t* index, const uint64_t* starts,
+                      const float* h0, void* y, float* final, float* carry, float* workspace, size_t workspace_floats, tf_stream_t stream);
+int tf_gated_scan_bwd(const TfGatedScan* d, const void* gate, const void* x, const int64_t* offsets, const int64_t* index, const uint64_t* starts,
+                      const float* h0, const float* carry, const void* gy, const float* gfinal, void* dgate, void* dx, float* dh0, float* workspace,
+                      size_t workspace_floats, tf_stream_t stream);
+
+/* One step of n_rows sequences whose states live in rows of state [n_slots, channels]: state[slots[r]] = a state[slots[r]] + b in place, y[r] the
+ * new state in x's type.  A row whose slot is outside [0, n_slots) is skipped (y[r] by zero_rest); rows of one slot are steps in their order.
+ * n_rows <= 65536; d->n_segments and d->reverse are not read. */
+int tf_gated_step(const TfGatedScan* d, const void* gate, const void* x, const int64_t* slots, int64_t n_slots, float* state, void* y, tf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * TensoFlow coupling flow ('pwquad', 2 blocks, n_bins = 10): network/flow.py:314-525, :549-641,
  * :766-855.  Net k (flows.k.nn.{1,3,5,7}): Linear 44->64->64->64->21, LeakyReLU(0.01), input
  * Reshift(2,-1).  cond [pn,37] = [nis feature 16 | embed3(view_angles) 14 | 0 x 7].

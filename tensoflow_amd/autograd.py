@@ -412,6 +412,38 @@ class CompositeFn(torch.autograd.Function):
         return ga, (gvs[0] if len(gvs) == 1 else torch.cat(gvs, -1)), None, None
 
 
+class GatedScanFn(torch.autograd.Function):
+    """(y, final) = the gated linear recurrence over a packed batch (tf_gated_scan_fwd); backward tf_gated_scan_bwd wrt gate, x and h0.  The
+    states are computed again in the backward pass, from x and the fp32 states kept every few rows: y may be rounded, its gradient is not."""
+
+    @staticmethod
+    def forward(ctx, gate, x, h0, tables, form, reverse):
+        d = lambda t: None if t is None else t.detach()
+        y, final, carry = ops.gated_scan(d(gate), d(x), tables, d(h0), form, reverse, want_final=tables.index is not None, want_carry=True)
+        ctx.save_for_backward(gate, x, h0, carry)
+        ctx.cfg = (tables, form, reverse)
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    def backward(ctx, gy, g_final):
+        gate, x, h0, carry = ctx.saved_tensors
+        tables, form, reverse = ctx.cfg
+        if gy is None and g_final is None:
+            return None, None, None, None, None, None
+        c = lambda t: None if t is None else t.contiguous()
+        need = ctx.needs_input_grad
+        g = ops.gated_scan_bwd(gate, x, tables, carry, c(gy), c(g_final), h0, form, reverse, need[0], need[1], need[2])
+        return (*g, None, None, None)
+
+
+def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False):
+    """Differentiable `ops.gated_scan` -> (y, final) (final None where the tables have no index).  Leaves that a captured graph and eager code
+    both use: take their gradients by torch.autograd.grad, not by accumulation into .grad."""
+    rows = lambda t: t if t.dim() < 2 or t[:1].is_contiguous() else t.contiguous()      # channels side by side; any row stride
+    return GatedScanFn.apply(rows(gate), rows(x), None if h0 is None else h0.contiguous(), tables, form, reverse)
+
+
 def sdf_alpha_composed(planes, lines, W1, b1, W2, b2, pts, level, dists, dirs, inv_s, cos_anneal, aabb, units, n_levels):
     """Differentiable restatement of tf_sdf_alpha_fwd used ONLY inside SdfAlphaFn.backward: the gather is the HIP kernel pair
     (VmGatherFn), the two decoder products are the HIP dense-layer kernels (LinearActFn) over all 7 taps, the rest is elementwise."""

@@ -51,6 +51,11 @@ class TfBvhNode(C.Structure):
     _fields_ = [("lo", f32 * 3), ("left", i32), ("hi", f32 * 3), ("count", i32)]
 
 
+class TfGatedScan(C.Structure):
+    _fields_ = [("n_rows", i64), ("n_segments", i64), ("ld_x", i64), ("ld_gate", i64), ("channels", i32), ("gates", i32),
+                ("x_type", i32), ("gate_type", i32), ("form", i32), ("reverse", i32), ("zero_rest", i32)]
+
+
 P = C.POINTER
 F3 = c_f * 3
 
@@ -75,6 +80,14 @@ SIGNATURES = {
                                    c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, i32, c_f, sz, c_f]),
     "tf_composite_fwd": (C.c_int, [c_f, c_f, c_f, i64, i64, i32, c_f, c_f, c_f, c_f]),
     "tf_composite_bwd": (C.c_int, [c_f, c_f, c_f, c_f, c_f, c_f, i64, i64, i32, c_f, c_f, c_f]),
+    "tf_segment_workspace_words": (sz, [i64, i64]),
+    "tf_segment_tables": (C.c_int, [c_f, i64, i64, c_f, c_f, c_f, c_f, i64, c_f, i64, i64, c_f, c_f, c_f, sz, c_f]),
+    "tf_segment_from_index": (C.c_int, [c_f, i64, i64, c_f, c_f, c_f]),
+    "tf_gated_scan_carry_floats": (sz, [P(TfGatedScan)]),
+    "tf_gated_scan_workspace_floats": (sz, [P(TfGatedScan), i32]),
+    "tf_gated_scan_fwd": (C.c_int, [P(TfGatedScan), c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, sz, c_f]),
+    "tf_gated_scan_bwd": (C.c_int, [P(TfGatedScan), c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, sz, c_f]),
+    "tf_gated_step": (C.c_int, [P(TfGatedScan), c_f, c_f, c_f, i64, c_f, c_f, c_f]),
     "tf_flow_workspace_floats": (sz, [i64]),
     "tf_flow_sample_fwd": (C.c_int, [P(TfCouplingNet * 2), c_f, c_f, c_f, i64, i32, c_f, c_f, c_f, i32, c_f, sz, c_f]),
     "tf_flow_logq_fwd": (C.c_int, [P(TfCouplingNet * 2), c_f, c_f, c_f, i64, i32, i64, c_f, c_f, c_f, i32, c_f, sz, c_f]),

@@ -514,6 +514,202 @@ def composite_bwd(alpha, ray_indices, values, weights, g_acc, g_out, n_rays):
     return g_alpha, g_values
 
 
+# ------------------------------------------------------------------------------ packed sequences
+class SegmentTables:
+    """Tables of a packed batch (built by `segment_tables` / `segment_tables_from_index`): offsets [R + 1], index [N] (= ray_indices), position [N],
+    starts [ceil(N / 64)] (one bit a row), block_table [R, M] and slots [N]; what was not asked for is None."""
+    __slots__ = ("n_rows", "n_segments", "offsets", "index", "position", "starts", "block_table", "slots")
+
+    def __init__(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None):
+        self.n_rows, self.n_segments, self.offsets, self.index, self.position = n_rows, n_segments, offsets, index, position
+        self.starts, self.block_table, self.slots = starts, block_table, slots
+
+
+def _on(*tensors):
+    """The stream to enqueue on: the current one of the tensors' device, which has to be the current device."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"tensors on {dev} and {t.device}: one device is wanted")
+    if dev.type != "cuda":
+        raise RuntimeError("a CUDA/HIP tensor is wanted (tensoflow_amd has no CPU path)")
+    if dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}: enter torch.cuda.device({dev.index})")
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_MOST_ROWS = 1 << 38
+
+
+def segment_offsets(lengths):
+    """Exclusive sums [R + 1] of the int64 lengths [R] of a packed batch (the first table of `segment_tables` alone; offsets[-1] rows in all)."""
+    if lengths.dim() != 1:
+        raise RuntimeError(f"lengths must be [R], got {tuple(lengths.shape)}")
+    stream = _on(lengths)
+    R, null = lengths.shape[0], C.c_void_p(0)
+    offsets = torch.empty(R + 1, dtype=torch.int64, device=lengths.device)
+    L.check(L.load().tf_segment_tables(_p(lengths, torch.int64, "lengths"), R, _MOST_ROWS, offsets.data_ptr(), null, null, null, 0, null, 0, 0, null, null, null,
+                                       0, stream), "tf_segment_tables")
+    return offsets
+
+
+def segment_tables(lengths, n_rows=None, index=True, position=True, block_rows=0, free_blocks=None, max_blocks=None):
+    """SegmentTables of the int64 lengths [R] of a packed batch.  n_rows: the number of rows (of the packed tensors); None: the lengths' sum, with one
+    host read.  Rows behind the last segment get index and position -1; lengths that sum to more are cut there.
+    block_rows > 0: also block_table [R, max_blocks] int32 and slots [N] of rows kept in blocks of a shared store, the blocks dealt in order from
+    free_blocks (int32; None: 0, 1, 2 ...); max_blocks: width of the table (None: as many as n_rows could need)."""
+    if lengths.dim() != 1:
+        raise RuntimeError(f"lengths must be [R], got {tuple(lengths.shape)}")
+    stream = _on(lengths, free_blocks)
+    R, dev = lengths.shape[0], lengths.device
+    pl = _p(lengths, torch.int64, "lengths")
+    if n_rows is None:
+        n_rows = int(segment_offsets(lengths)[-1])
+    if n_rows < 0 or block_rows < 0:
+        raise RuntimeError("n_rows and block_rows must not be negative")
+    new = lambda *s, dtype=torch.int64: torch.empty(s, dtype=dtype, device=dev)
+    t = SegmentTables(n_rows, R, new(R + 1), new(n_rows) if index else None, new(n_rows) if position else None, new((n_rows + 63) // 64))
+    lib, work, n_free = L.load(), None, 0
+    if block_rows:
+        if free_blocks is None:
+            free_blocks = torch.arange(n_rows // block_rows + R, dtype=torch.int32, device=dev)
+        n_free = free_blocks.numel()
+        max_blocks = (n_rows + block_rows - 1) // block_rows if max_blocks is None else max_blocks
+        t.block_table, t.slots = new(R, max_blocks, dtype=torch.int32), new(n_rows)
+        work = new(lib.tf_segment_workspace_words(R, block_rows))
+    elif free_blocks is not None or max_blocks:
+        raise RuntimeError("free_blocks and max_blocks go with block_rows")
+    L.check(lib.tf_segment_tables(pl, R, n_rows, t.offsets.data_ptr(), _p(t.index, torch.int64), _p(t.position, torch.int64), t.starts.data_ptr(),
+                                  block_rows, _p(free_blocks, torch.int32, "free_blocks"), n_free, max_blocks or 0, _p(t.block_table, torch.int32),
+                                  _p(t.slots, torch.int64), _p(work, torch.int64), 0 if work is None else work.numel(), stream), "tf_segment_tables")
+    return t
+
+
+def segment_tables_from_index(index, n_segments):
+    """SegmentTables (offsets, starts) of a sorted int64 index [N], the ray_indices of a packed sampler."""
+    if index.dim() != 1:
+        raise RuntimeError(f"index must be [N], got {tuple(index.shape)}")
+    stream = _on(index)
+    pi = _p(index, torch.int64, "index")
+    n, dev = index.shape[0], index.device
+    t = SegmentTables(n, n_segments, torch.empty(n_segments + 1, dtype=torch.int64, device=dev), index, None,
+                      torch.empty((n + 63) // 64, dtype=torch.int64, device=dev))
+    L.check(L.load().tf_segment_from_index(pi, n, n_segments, t.offsets.data_ptr(), t.starts.data_ptr(), stream), "tf_segment_from_index")
+    return t
+
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}                    # TfType
+_GATE_FORMS = {"decay": 0, "log": 1, "alpha": 2}                                    # TfGateForm
+
+
+def _rows_of(t, name):
+    """(rows, channels, row stride) of a [N], [N, C] or [N, H, P] tensor whose channels stand side by side."""
+    if t.dtype not in _TYPES:
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 1:
+        return shape[0], 1, stride[0]
+    width = 1
+    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if n != 1 and s != width and t.numel():
+            raise RuntimeError(f"{name} must be contiguous in its channels, got strides {stride}")
+        width *= n
+    return shape[0], width, stride[0]
+
+
+def _scan_desc(gate, x, n_segments, form, reverse, zero_rest):
+    if form not in _GATE_FORMS:
+        raise RuntimeError(f"form must be one of {sorted(_GATE_FORMS)}, got {form!r}")
+    if x.dim() < 2 or gate.dim() < 1:
+        raise RuntimeError("x must be [N, C] or [N, H, P], the gate [N] or with channels")
+    n, c, ldx = _rows_of(x, "x")
+    ng, g, ldg = _rows_of(gate, "gate")
+    if ng != n or g < 1 or c < 1 or c % g:
+        raise RuntimeError(f"a gate {tuple(gate.shape)} does not go with x {tuple(x.shape)}: as many rows, and channels that divide x's")
+    if gate.dtype != x.dtype and gate.dtype != torch.float32:
+        raise RuntimeError(f"the gate must be {x.dtype} or float32, got {gate.dtype}")
+    return L.TfGatedScan(n, n_segments, ldx, ldg, c, g, _TYPES[x.dtype], _TYPES[gate.dtype], _GATE_FORMS[form], 1 if reverse else 0, zero_rest), n, c
+
+
+def _like_x(t, x, name):
+    if t.shape != x.shape or t.dtype != x.dtype:
+        raise RuntimeError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
+    return _p(t, x.dtype, name)
+
+
+def _state(t, n, c, name):
+    if t is not None and (t.shape[:1] != (n,) or t.numel() != n * c):
+        raise RuntimeError(f"{name} must be [{n}, {c}], got {tuple(t.shape)}")
+    return _p(t, torch.float32, name)
+
+
+def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final=False, out=None, want_carry=False):
+    """h_t = a_t h_{t-1} + b_t along every segment of `tables` -> (y, final): y like x holds every h_t, final [R, C] fp32 the last ones (None unless
+    wanted).  form "decay": a = gate, b = x; "log": a = exp(gate), b = x; "alpha": a = 1 - gate, b = gate x.  x [N, C] (or [N, H, P]) fp32 / fp16 / bf16;
+    gate [N], [N, G] or like x, of x's type or fp32, each serving C / G consecutive channels.  h0 [R, C] fp32: the states before the first step.  reverse: from
+    each segment's last row to its first.  out: written in x's place of y, rows of no segment left as they are (without it they are 0).
+    want_carry: -> (y, final, carry) for `gated_scan_bwd`."""
+    stream = _on(x, gate, h0, out, tables.offsets)
+    R = tables.n_segments
+    d, n, c = _scan_desc(gate, x, R, form, reverse, 1 if out is None else 0)
+    if n != tables.n_rows:
+        raise RuntimeError(f"x has {n} rows, the tables {tables.n_rows}")
+    if tables.index is None and (h0 is not None or want_final):
+        raise RuntimeError("h0 and final need tables with an index")
+    ph = _state(h0, R, c, "h0")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    py = _like_x(y, x, "out")
+    new = lambda k: torch.empty(k, dtype=torch.float32, device=x.device) if k else None
+    final = torch.empty(R, *x.shape[1:], dtype=torch.float32, device=x.device) if want_final else None
+    lib = L.load()
+    carry = torch.empty(lib.tf_gated_scan_carry_floats(C.byref(d)), dtype=torch.float32, device=x.device) if want_carry else None
+    nw = lib.tf_gated_scan_workspace_floats(C.byref(d), 0)
+    work = new(nw)
+    L.check(lib.tf_gated_scan_fwd(C.byref(d), gate.data_ptr(), x.data_ptr(), tables.offsets.data_ptr(), _p(tables.index, torch.int64), tables.starts.data_ptr(),
+                                  ph, py, _p(final), _p(carry), _p(work), nw, stream), "tf_gated_scan_fwd")
+    return (y, final, carry) if want_carry else (y, final)
+
+
+def gated_scan_bwd(gate, x, tables, carry, gy, g_final, h0=None, form="decay", reverse=False, need_gate=True, need_x=True, need_h0=True):
+    """Gradients of `gated_scan` -> (g_gate, g_x, g_h0) (None where not needed); carry: what the forward pass kept; gy like x and g_final [R, C] may be None."""
+    stream = _on(x, gate, h0, carry, gy, g_final, tables.offsets)
+    R = tables.n_segments
+    d, n, c = _scan_desc(gate, x, R, form, reverse, 1)
+    if n != tables.n_rows:
+        raise RuntimeError(f"x has {n} rows, the tables {tables.n_rows}")
+    if tables.index is None and (h0 is not None or g_final is not None or need_h0):
+        raise RuntimeError("h0 and final need tables with an index")
+    lib = L.load()
+    if carry.numel() != lib.tf_gated_scan_carry_floats(C.byref(d)):
+        raise RuntimeError("carry is not of this scan")
+    ph, pf = _state(h0, R, c, "h0"), _state(g_final, R, c, "g_final")
+    pg = C.c_void_p(0) if gy is None else _like_x(gy, x, "gy")
+    new = lambda like, ok: torch.empty(like.shape, dtype=like.dtype, device=x.device) if ok else None
+    g_gate, g_x = new(gate, need_gate), new(x, need_x)
+    g_h0 = torch.empty(R, *x.shape[1:], dtype=torch.float32, device=x.device) if need_h0 else None
+    nw = lib.tf_gated_scan_workspace_floats(C.byref(d), 1)
+    work = torch.empty(nw, dtype=torch.float32, device=x.device) if nw else None
+    L.check(lib.tf_gated_scan_bwd(C.byref(d), gate.data_ptr(), x.data_ptr(), tables.offsets.data_ptr(), _p(tables.index, torch.int64), tables.starts.data_ptr(),
+                                  ph, _p(carry), pg, pf, _p(g_gate, gate.dtype), _p(g_x, x.dtype), _p(g_h0), _p(work), nw, stream), "tf_gated_scan_bwd")
+    return g_gate, g_x, g_h0
+
+
+def gated_step(state, slots, gate, x, form="decay", out=None):
+    """One step of B sequences: state[slots[r]] = a state[slots[r]] + b in place (fp32 pool [S, C], slots int64 [B]) -> y like x, the new states.
+    Gates and forms as in `gated_scan`.  Rows with a slot outside the pool are skipped (their y is 0, or as in `out`); rows that share a slot
+    are consecutive steps of it."""
+    stream = _on(x, gate, state, slots, out)
+    d, n, c = _scan_desc(gate, x, 0, form, False, 1 if out is None else 0)
+    if slots.shape != (n,):
+        raise RuntimeError(f"slots must be [{n}], got {tuple(slots.shape)}")
+    if state.dim() < 2 or state.shape[1:].numel() != c:
+        raise RuntimeError(f"state must be [S, {c}], got {tuple(state.shape)}")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    L.check(L.load().tf_gated_step(C.byref(d), gate.data_ptr(), x.data_ptr(), _p(slots, torch.int64, "slots"), state.shape[0],
+                                   _p(state, torch.float32, "state"), _like_x(y, x, "out"), stream), "tf_gated_step")
+    return y
+
+
 # ------------------------------------------------------------------------------ flow
 def _coupling_nets(weights):
     """weights: list of 2 lists of 4 (W, b) pairs."""
@@ -888,9 +1084,8 @@ def march_uniform(o, d, near, far, aabb, n_steps, step_size=0.0, volume_u8=None,
     tj = _p(_f(t_jitter.reshape(-1))) if t_jitter is not None else None
     L.check(lib.tf_march_uniform(_p(o), _p(d), _p(near), _p(far), rn, n_steps, float(step_size), C.byref(box), vol, D, H, W,
                                  C.byref(mbox), mode, tj, null, _p(counts, torch.int64), null, null, null, _stream()), "tf_march_uniform")
-    incl = torch.cumsum(counts, 0)
-    offsets = (incl - counts).contiguous()
-    n = int(incl[-1]) if rn > 0 else 0
+    offsets = segment_offsets(counts)
+    n = int(offsets[-1])
     t0 = torch.empty(n, dtype=torch.float32, device=dev)
     t1 = torch.empty(n, dtype=torch.float32, device=dev)
     ridx = torch.empty(n, dtype=torch.int64, device=dev)
