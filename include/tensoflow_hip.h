@@ -202,7 +202,7 @@ int tf_composite_bwd(const float* alpha, const int64_t* ray_indices, const float
  * tf_segment_tables: from lengths[n_segments] (values below 0 count as 0, above n_rows as n_rows)
  *   offsets[n_segments + 1] = exclusive sums, cut at n_rows;  index[i] = the segment of row i (ray_indices);
  *   position[i] = i - offsets[index[i]];  bit i % 64 of starts[i / 64] = row i is a segment's first ((n_rows + 63) / 64 words).
- *   Rows behind the last segment have index and position -1 and no start bit.  index, position, starts may be NULL.
+ *   Rows behind the last segment have index and position -1 and no start bit.  index, position (and starts where neither is wanted) may be NULL; slots need index.
  *   block_rows > 0: the rows of segment s live in blocks of block_rows rows of a shared store; its c-th block is
  *   block_table[s, c] = free_blocks[sum_{q<s} ceil(lengths[q] / block_rows) + c], -1 behind its last block or the list's end;
  *   slots[i] = block * block_rows + position % block_rows, -1 where there is no block or it lies behind max_blocks.
@@ -251,7 +251,7 @@ int tf_gated_scan_bwd(const TfGatedScan* d, const void* gate, const void* x, con
 
 /* One step of n_rows sequences whose states live in rows of state [n_slots, channels]: state[slots[r]] = a state[slots[r]] + b in place, y[r] the
  * new state in x's type.  A row whose slot is outside [0, n_slots) is skipped (y[r] by zero_rest); rows of one slot are steps in their order.
- * n_rows <= 65536; d->n_segments and d->reverse are not read. */
+ * n_rows <= 8192; d->n_segments and d->reverse are not read. */
 int tf_gated_step(const TfGatedScan* d, const void* gate, const void* x, const int64_t* slots, int64_t n_slots, float* state, void* y, tf_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------

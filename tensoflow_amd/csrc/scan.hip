@@ -630,32 +630,56 @@ __global__ void __launch_bounds__(256) scan_clear_kernel(ull* __restrict__ words
   if (i == 0) *ticket = 0;
 }
 
-// one thread per (row, channel): the first row of a slot takes the later ones of the same slot along, in order
-template <typename XT, typename GT>
-__global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, const GT* __restrict__ gate, const XT* __restrict__ x, const ll* __restrict__ slots,
+// A workgroup is a row and 256 V of its channels.  The first row of a slot takes the later ones of the same slot along, in order; the others leave.
+template <typename XT, typename GT, int V, bool SHARED>
+__global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, const GT* __restrict__ gate, const XT* __restrict__ x, const ll* __restrict__ slots,
                                                    ll n_slots, float* __restrict__ state, XT* __restrict__ y) {
-  const ll e = (ll)blockIdx.x * 256 + threadIdx.x;
-  const int D = d.channels, P = D / d.gates;
-  const ll r = e / D;
-  if (r >= d.n_rows) return;
-  const int c = (int)(e % D);
+  constexpr int AV = SHARED ? 1 : V;
+  const int D = d.channels, P = D / d.gates, n = (int)d.n_rows, r = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * V;
+  const bool mine = c < D;
   const ll slot = slots[r];
   if (slot < 0 || slot >= n_slots) {
-    if (d.zero_rest) y[e] = from_f<XT>(0.f);
+    const float z[V] = {};
+    if (d.zero_rest && mine) store_v<XT, V>(y + (ll)r * D + c, z, aligned);
     return;
   }
-  for (ll q = 0; q < r; ++q)
-    if (slots[q] == slot) return;
-  float h = state[slot * D + c];
-  for (ll q = r; q < d.n_rows; ++q) {
-    if (slots[q] != slot) continue;
-    float a = to_f(gate[q * d.ld_gate + c / P]), b = to_f(x[q * d.ld_x + c]);
-    if (d.form == TF_GATE_LOG) a = exp_gate(a);
-    if (d.form == TF_GATE_ALPHA) b *= a, a = 1.f - a;
-    h = fmaf(a, h, b);
-    y[q * D + c] = from_f<XT>(h);
+  const ll g = SHARED ? c / P : c;
+  Vec<XT, V> rx;
+  Vec<GT, AV> rg;
+  Vec<float, V> h;
+  if (mine) {  // asked for before the search, which needs none of it
+    rx = load_v<XT, V>(x + r * d.ld_x + c, aligned);
+    rg = load_v<GT, AV>(gate + r * d.ld_gate + g, aligned);
+    h = load_v<float, V>(state + slot * D + c, aligned);
   }
-  state[slot * D + c] = h;
+  int last = r;
+  if (n > 1) {
+    int before = 0, behind = 0;
+    for (int q = threadIdx.x; q < n; q += 256) {
+      const bool same = slots[q] == slot;
+      before |= same && q < r;
+      behind |= same && q > r;
+    }
+    if (__syncthreads_or(before)) return;
+    if (__syncthreads_or(behind)) last = n - 1;
+  }
+  if (!mine) return;
+  for (int q = r; q <= last; ++q) {
+    if (q != r) {
+      if (slots[q] != slot) continue;
+      rx = load_v<XT, V>(x + q * d.ld_x + c, aligned);
+      rg = load_v<GT, AV>(gate + q * d.ld_gate + g, aligned);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float a = to_f(rg.v[AV == 1 ? 0 : v]), b = to_f(rx.v[v]);
+      if (d.form == TF_GATE_LOG) a = exp_gate(a);
+      if (d.form == TF_GATE_ALPHA) b *= a, a = 1.f - a;
+      h.v[v] = fmaf(a, h.v[v], b);
+    }
+    store_v<XT, V>(y + (ll)q * D + c, h.v, aligned);
+  }
+  store_v<float, V>(state + slot * D + c, h.v, aligned);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -863,17 +887,28 @@ extern "C" int tf_gated_scan_bwd(const TfGatedScan* d, const void* gate, const v
 extern "C" int tf_gated_step(const TfGatedScan* d, const void* gate, const void* x, const int64_t* slots, int64_t n_slots, float* state, void* y,
                              tf_stream_t stream) {
   if (int rc = check_desc(d, "tf_gated_step")) return rc;
-  TF_REQUIRE(n_slots >= 0 && d->n_rows <= 65536, TF_ESHAPE, "tf_gated_step: a negative pool size, or over 65536 rows");
+  TF_REQUIRE(n_slots >= 0 && d->n_rows <= 8192, TF_ESHAPE, "tf_gated_step: a negative pool size, or over 8192 rows");
   if (d->n_rows == 0) return TF_OK;
   TF_REQUIRE(gate && x && slots && y && (n_slots == 0 || state), TF_EINVAL, "tf_gated_step: null pointer");
-  const unsigned blocks = (unsigned)((d->n_rows * (ll)d->channels + 255) / 256);
+  // four channels a lane, unless that leaves most of the card idle: one row of 2048 channels is 8 workgroups at one channel a lane
+  const bool shared = d->channels != d->gates;
+  const int unit = shared ? d->channels / d->gates : d->channels;
+  const int V = unit % 4 == 0 && d->n_rows * d->channels >= 65536 ? 4 : 1;
+  const size_t xs = d->x_type == TF_TYPE_F32 ? 4 : 2, gs = d->gate_type == TF_TYPE_F32 ? 4 : 2;
+  const int vg = shared ? 1 : V;
+  const int aligned = fits(x, V * xs) && fits(y, V * xs) && fits(gate, vg * gs) && fits(state, V * 4) && (d->n_rows == 1 || (d->ld_x % V == 0 && d->ld_gate % vg == 0));
+  const dim3 grid((unsigned)((d->channels + 256 * V - 1) / (256 * V)), (unsigned)d->n_rows);
   hipStream_t st = (hipStream_t)stream;
-#define STEP(XT, GT) step_kernel<XT, GT><<<blocks, 256, 0, st>>>(*d, static_cast<const GT*>(gate), static_cast<const XT*>(x), (const ll*)slots, n_slots, state, static_cast<XT*>(y))
-  if (d->x_type == TF_TYPE_F32) STEP(float, float);
-  else if (d->x_type == TF_TYPE_F16 && d->gate_type == TF_TYPE_F16) STEP(__half, __half);
-  else if (d->x_type == TF_TYPE_F16) STEP(__half, float);
-  else if (d->gate_type == TF_TYPE_BF16) STEP(__hip_bfloat16, __hip_bfloat16);
-  else STEP(__hip_bfloat16, float);
+#define STEP(XT, GT, VV, SH) step_kernel<XT, GT, VV, SH><<<grid, 256, 0, st>>>(*d, aligned, static_cast<const GT*>(gate), static_cast<const XT*>(x), (const ll*)slots, n_slots, state, static_cast<XT*>(y))
+#define STEP_V(XT, GT)                                                            \
+  if (V == 4) { if (shared) STEP(XT, GT, 4, true); else STEP(XT, GT, 4, false); } \
+  else { if (shared) STEP(XT, GT, 1, true); else STEP(XT, GT, 1, false); }
+  if (d->x_type == TF_TYPE_F32) { STEP_V(float, float) }
+  else if (d->x_type == TF_TYPE_F16 && d->gate_type == TF_TYPE_F16) { STEP_V(__half, __half) }
+  else if (d->x_type == TF_TYPE_F16) { STEP_V(__half, float) }
+  else if (d->gate_type == TF_TYPE_BF16) { STEP_V(__hip_bfloat16, __hip_bfloat16) }
+  else { STEP_V(__hip_bfloat16, float) }
+#undef STEP_V
 #undef STEP
   TF_LAUNCH_CHECK("tf_gated_step");
   return TF_OK;

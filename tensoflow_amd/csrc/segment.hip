@@ -1,6 +1,7 @@
 // Tables of a packed batch of sequences, built on the device from their lengths (or from a sorted segment index):
 //   offsets[s] = sum_{q<s} len[q], index[i] = the segment of row i, position[i] = i - offsets[index[i]], bit i of `starts` = position[i] == 0,
-// and, for rows kept in blocks of B rows of a shared store: request s owns blocks first[s] .. first[s] + ceil(len[s] / B) of the free list.
+// and, for rows kept in blocks of B rows of a shared store: segment s owns entries first[s] .. first[s] + ceil(len[s] / B) of the free list.
+// Bound: the launch for a batch, the writes (8 bytes a row and table) for a frame.
 #include "tf_common.h"
 
 namespace {
@@ -8,79 +9,228 @@ namespace {
 typedef long long ll;
 typedef unsigned long long ull;
 
+// Up to SMALL segments every workgroup sums the lengths by itself and finds its rows' segments in LDS: ONE launch, where the sums' own would cost
+// as much again (1024 segments, 130003 rows: 9.6 -> 6.4 us of kernels).  More segments: sums, offsets, rows.
+constexpr int SMALL = 2048;
+constexpr int CHUNK = 4096;  // lengths of a workgroup of the sums
+constexpr int WAVE_ROWS = 512;
+
 __device__ __forceinline__ ll seg_len(const ll* __restrict__ lengths, ll s, ll n_rows) { return min(max(lengths[s], 0ll), n_rows); }
 
-// first segment whose END lies beyond row i: the segment that holds it (empty ones end where they begin and are passed over)
-__device__ __forceinline__ ll seg_of_row(const ll* __restrict__ offsets, ll n_seg, ll i) {
-  ll lo = 0, hi = n_seg;
-  while (lo < hi) {
-    const ll mid = (lo + hi) >> 1;
-    if (offsets[mid + 1] <= i) lo = mid + 1; else hi = mid;
+struct Blocks {
+  ll rows, n_free, max_blocks;
+  const int* free_blocks;
+  int* table;
+  ll* slots;
+  int shift;  // log2(rows), or -1
+};
+__device__ __forceinline__ ll blocks_of(const Blocks& b, ll n) { return b.shift >= 0 ? (n + b.rows - 1) >> b.shift : (n + b.rows - 1) / b.rows; }
+__device__ __forceinline__ ll slot_of(const Blocks& b, ll first, ll pos) {
+  const ll c = b.shift >= 0 ? pos >> b.shift : pos / b.rows;
+  if (c >= b.max_blocks || first + c >= b.n_free) return -1;
+  const ll blk = b.free_blocks[first + c];
+  return blk < 0 ? -1 : blk * b.rows + (pos - c * b.rows);
+}
+
+__device__ __forceinline__ ll wave_inclusive(ll v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const ll p = __shfl_up(v, o);
+    if (lane >= o) v += p;
+  }
+  return v;
+}
+// exclusive sums over the workgroup's threads; `total` of all of them
+template <int WAVES>
+__device__ __forceinline__ ll block_exclusive(ll v, ll* part, ll& total) {
+  const int wave = threadIdx.x >> 6;
+  const ll in = wave_inclusive(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) part[wave] = in;
+  __syncthreads();
+  ll before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) before += part[w];
+    total += part[w];
+  }
+  return before + in - v;
+}
+
+__global__ void __launch_bounds__(256) seg_small_kernel(const ll* __restrict__ lengths, int n_seg, ll n_rows, ll rows_per_block, ll* __restrict__ offsets,
+                                                        ll* __restrict__ index, ll* __restrict__ position, ull* __restrict__ starts, Blocks b) {
+  __shared__ ll off[SMALL + 1], first[SMALL], part[4];
+  constexpr int PER = SMALL / 256;
+  const int t = threadIdx.x;
+  ll v[PER], sum = 0, bsum = 0, total, btotal;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int s = t * PER + k;
+    v[k] = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
+    sum += v[k];
+    if (b.rows) bsum += blocks_of(b, v[k]);
+  }
+  ll at = block_exclusive<4>(sum, part, total), bat = b.rows ? block_exclusive<4>(bsum, part, btotal) : 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int s = t * PER + k;
+    if (s < n_seg) {
+      off[s] = min(at, n_rows);
+      if (b.rows) first[s] = bat;
+    }
+    at += v[k];
+    if (b.rows) bat += blocks_of(b, v[k]);
+  }
+  if (t == 0) off[n_seg] = min(total, n_rows);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int s = t; s <= n_seg; s += 256) offsets[s] = off[s];
+  if (b.table) {
+    const ll n = n_seg * b.max_blocks;
+    for (ll e = (ll)blockIdx.x * 256 + t; e < n; e += (ll)gridDim.x * 256) {
+      const int s = n < (1ll << 31) ? (int)((unsigned)e / (unsigned)b.max_blocks) : (int)(e / b.max_blocks);
+      const ll c = e - s * b.max_blocks;
+      b.table[e] = c < blocks_of(b, seg_len(lengths, s, n_rows)) && first[s] + c < b.n_free ? b.free_blocks[first[s] + c] : -1;
+    }
+  }
+  if (!starts) return;
+  const ll r1 = min(n_rows, (blockIdx.x + 1) * rows_per_block), end = off[n_seg];
+  for (ll base = blockIdx.x * rows_per_block; base < r1; base += 256) {
+    const ll i = base + t;
+    // the first segment whose END lies beyond row i: the one that holds it (empty ones end where they begin and are passed over)
+    int lo = 0, hi = n_seg;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (off[mid + 1] <= i) lo = mid + 1; else hi = mid;
+    }
+    const bool ok = i < end;
+    const ll p = ok ? i - off[lo] : -1;
+    const ull bits = __ballot(p == 0);
+    if (i < r1) {
+      if ((t & 63) == 0) starts[i >> 6] = bits;
+      if (index) index[i] = ok ? lo : -1;
+      if (position) position[i] = p;
+      if (b.slots) b.slots[i] = ok ? slot_of(b, first[lo], p) : -1;
+    }
+  }
+}
+
+// sums of CHUNK lengths (and of their block counts); the start bits cleared
+__global__ void __launch_bounds__(256) seg_sums_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, Blocks b, ll* __restrict__ sums,
+                                                       ull* __restrict__ starts, ll n_words) {
+  __shared__ ll part[4];
+  const ll s0 = (ll)blockIdx.x * CHUNK;
+  ll sum = 0, bsum = 0, total;
+#pragma unroll
+  for (int k = 0; k < CHUNK / 256; ++k) {
+    const ll s = s0 + k * 256 + threadIdx.x;
+    if (s < n_seg) {
+      const ll v = seg_len(lengths, s, n_rows);
+      sum += v;
+      if (b.rows) bsum += blocks_of(b, v);
+    }
+  }
+  block_exclusive<4>(sum, part, total);
+  if (threadIdx.x == 0) sums[2 * blockIdx.x] = total;
+  if (b.rows) block_exclusive<4>(bsum, part, total);
+  if (threadIdx.x == 0) sums[2 * blockIdx.x + 1] = b.rows ? total : 0;
+  if (starts)
+    for (ll w = (ll)blockIdx.x * 256 + threadIdx.x; w < n_words; w += (ll)gridDim.x * 256) starts[w] = 0;
+}
+
+// offsets from the sums; every segment with rows marks its first one: the start bit, and its number in index
+__global__ void __launch_bounds__(256) seg_offsets_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, Blocks b, const ll* __restrict__ sums,
+                                                          ll* __restrict__ offsets, ll* __restrict__ block_first, ll* __restrict__ index, ull* __restrict__ starts) {
+  __shared__ ll part[4];
+  ll base = 0, bbase = 0, total;
+  for (ll c = threadIdx.x; c < blockIdx.x; c += 256) {
+    base += sums[2 * c];
+    bbase += sums[2 * c + 1];
+  }
+  block_exclusive<4>(base, part, total);
+  base = total;
+  block_exclusive<4>(bbase, part, total);
+  bbase = total;
+  for (int k = 0; k < CHUNK / 256; ++k) {
+    const ll s = (ll)blockIdx.x * CHUNK + k * 256 + threadIdx.x;
+    const ll v = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
+    const ll at = min(base + block_exclusive<4>(v, part, total), n_rows);
+    base += total;
+    ll bat = 0;
+    if (b.rows) {
+      bat = bbase + block_exclusive<4>(blocks_of(b, v), part, total);
+      bbase += total;
+    }
+    if (s >= n_seg) continue;
+    offsets[s] = at;
+    if (b.rows) block_first[s] = bat;
+    if (s == n_seg - 1) offsets[n_seg] = min(at + v, n_rows);
+    if (starts && v > 0 && at < n_rows) {
+      atomicOr(starts + (at >> 6), 1ull << (at & 63));
+      if (index) index[at] = s;
+    }
+  }
+}
+
+// the segment that holds row i < offsets[n_seg], by all lanes: 64 probes a round
+__device__ __forceinline__ ll wave_seg_of(const ll* __restrict__ offsets, ll n_seg, ll i) {
+  const int lane = threadIdx.x & 63;
+  ll lo = 0, n = n_seg;
+  while (n > 1) {
+    const ll step = (n + 63) >> 6, at = lo + lane * step + step - 1;
+    const ull hit = __ballot(at >= lo + n - 1 || offsets[at + 1] > i);
+    const int f = __ffsll((long long)hit) - 1;
+    lo += f * step;
+    n = min(step, n - f * step);
   }
   return lo;
 }
 
-// exclusive sums of the lengths and of the block counts: one workgroup walks the list
-__global__ void __launch_bounds__(1024) seg_sums_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, ll block_rows, ll* __restrict__ offsets,
-                                                        ll* __restrict__ block_first) {
-  __shared__ ll part[2][1024];
-  const int t = threadIdx.x;
-  ll base = 0, bbase = 0;
-  for (ll s0 = 0; s0 < n_seg; s0 += 1024) {
-    const ll s = s0 + t;
-    const ll v = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
-    const ll b = block_rows ? (v + block_rows - 1) / block_rows : 0;
-    part[0][t] = v;
-    part[1][t] = b;
-    __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {
-      const ll p = t >= o ? part[0][t - o] : 0, q = t >= o ? part[1][t - o] : 0;
-      __syncthreads();
-      part[0][t] += p;
-      part[1][t] += q;
-      __syncthreads();
-    }
-    if (s < n_seg) {
-      offsets[s] = min(base + part[0][t] - v, n_rows);
-      if (block_rows) block_first[s] = bbase + part[1][t] - b;
-    }
-    base += part[0][1023];
-    bbase += part[1][1023];
-    __syncthreads();
+// every row from the start bits: a row belongs to the last start at or before it, within its 64 rows or carried from before
+__global__ void __launch_bounds__(256) seg_rows_kernel(const ll* __restrict__ offsets, const ll* __restrict__ block_first, ll n_seg, ll n_rows,
+                                                       const ull* __restrict__ starts, ll* index, ll* __restrict__ position, Blocks b) {
+  constexpr int N = WAVE_ROWS / 64;
+  const int lane = threadIdx.x & 63;
+  const ll row0 = ((ll)blockIdx.x * 4 + (threadIdx.x >> 6)) * WAVE_ROWS, end = offsets[n_seg];
+  if (row0 >= n_rows) return;
+  ull word[N];
+  ll seg[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) word[k] = row0 + 64 * k < n_rows ? starts[(row0 >> 6) + k] : 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) seg[k] = index && (word[k] >> lane & 1) ? index[row0 + 64 * k + lane] : 0;
+  ll cseg = -1, cstart = 0;
+  if (!(word[0] & 1) && row0 < end) {
+    cseg = wave_seg_of(offsets, n_seg, row0);
+    cstart = offsets[cseg];
   }
-  if (t == 0) offsets[n_seg] = min(base, n_rows);
-}
-
-__global__ void __launch_bounds__(256) seg_rows_kernel(const ll* __restrict__ offsets, const int* __restrict__ table, ll n_seg, ll n_rows, ll block_rows,
-                                                       ll max_blocks, ll* __restrict__ index, ll* __restrict__ position, ull* __restrict__ starts,
-                                                       ll* __restrict__ slots) {
-  const ll i = (ll)blockIdx.x * 256 + threadIdx.x;
-  const bool in = i < n_rows;
-  const ll s = in ? seg_of_row(offsets, n_seg, i) : n_seg;
-  const bool ok = s < n_seg;
-  const ll p = ok ? i - offsets[s] : -1;
-  const ull bits = __ballot(p == 0);
-  if (!in) return;
-  if (index) index[i] = ok ? s : -1;
-  if (position) position[i] = p;
-  if (starts && (threadIdx.x & 63) == 0) starts[i >> 6] = bits;
-  if (slots) {
-    ll v = -1;
-    if (ok && p / block_rows < max_blocks) {
-      const int blk = table[s * max_blocks + p / block_rows];
-      if (blk >= 0) v = blk * block_rows + p % block_rows;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const ll i = row0 + 64 * k + lane;
+    const ull upto = word[k] & (~0ull >> (63 - lane));
+    const int src = upto ? 63 - __clzll((long long)upto) : 0, lastsrc = word[k] ? 63 - __clzll((long long)word[k]) : 0;
+    const ll near = __shfl(seg[k], src), lastseg = __shfl(seg[k], lastsrc);
+    const ll s = upto ? near : cseg, p = i - (upto ? row0 + 64 * k + src : cstart);
+    if (word[k]) {
+      cseg = lastseg;
+      cstart = row0 + 64 * k + lastsrc;
     }
-    slots[i] = v;
+    if (i < n_rows) {
+      const bool ok = i < end;
+      if (index) index[i] = ok ? s : -1;
+      if (position) position[i] = ok ? p : -1;
+      if (b.slots) b.slots[i] = ok ? slot_of(b, block_first[s], p) : -1;
+    }
   }
 }
 
-__global__ void __launch_bounds__(256) seg_blocks_kernel(const ll* __restrict__ lengths, const ll* __restrict__ block_first, const int* __restrict__ free_blocks,
-                                                         ll n_free, ll n_seg, ll n_rows, ll block_rows, ll max_blocks, int* __restrict__ table) {
-  const ll e = (ll)blockIdx.x * 256 + threadIdx.x;
-  if (e >= n_seg * max_blocks) return;
-  const ll s = e / max_blocks, c = e % max_blocks;
-  const ll have = (seg_len(lengths, s, n_rows) + block_rows - 1) / block_rows, at = block_first[s] + c;
-  table[e] = c < have && at < n_free ? free_blocks[at] : -1;
+__global__ void __launch_bounds__(256) seg_blocks_kernel(const ll* __restrict__ lengths, const ll* __restrict__ block_first, ll n_seg, ll n_rows, Blocks b) {
+  const ll e = (ll)blockIdx.x * 256 + threadIdx.x, n = n_seg * b.max_blocks;
+  if (e >= n) return;
+  const ll s = n < (1ll << 31) ? (ll)((unsigned)e / (unsigned)b.max_blocks) : e / b.max_blocks, c = e - s * b.max_blocks, at = block_first[s] + c;
+  b.table[e] = c < blocks_of(b, seg_len(lengths, s, n_rows)) && at < b.n_free ? b.free_blocks[at] : -1;
 }
 
 // first row of a sorted index that is >= s
@@ -104,11 +254,13 @@ __global__ void __launch_bounds__(256) seg_starts_kernel(const ll* __restrict__ 
 }
 
 inline bool grid_fits(ll n, ll per) { return (n + per - 1) / per < (1ll << 31); }
+inline ll chunks_of(ll n_seg) { return (n_seg + CHUNK - 1) / CHUNK; }
 
 }  // namespace
 
 extern "C" size_t tf_segment_workspace_words(int64_t n_segments, int64_t block_rows) {
-  return block_rows > 0 && n_segments > 0 ? (size_t)n_segments : 0;
+  if (n_segments <= SMALL) return 0;
+  return 2 * (size_t)chunks_of(n_segments) + (block_rows > 0 ? (size_t)n_segments : 0);
 }
 
 extern "C" int tf_segment_tables(const int64_t* lengths, int64_t n_segments, int64_t n_rows, int64_t* offsets, int64_t* index, int64_t* position,
@@ -117,23 +269,41 @@ extern "C" int tf_segment_tables(const int64_t* lengths, int64_t n_segments, int
   TF_REQUIRE(n_segments >= 0 && n_rows >= 0 && block_rows >= 0 && n_free >= 0 && max_blocks >= 0, TF_ESHAPE, "tf_segment_tables: negative size");
   TF_REQUIRE(grid_fits(n_rows, 256) && grid_fits(n_segments, 256), TF_ESHAPE, "tf_segment_tables: too many rows or segments");
   TF_REQUIRE(offsets && (n_segments == 0 || lengths), TF_EINVAL, "tf_segment_tables: null pointer");
+  TF_REQUIRE(n_rows == 0 || starts || (!index && !position && !slots), TF_EINVAL, "tf_segment_tables: tables of rows need starts");
   const bool blocks = block_rows > 0;
   TF_REQUIRE(blocks || (!block_table && !slots), TF_EINVAL, "tf_segment_tables: block outputs without a block size");
   if (blocks) {
-    TF_REQUIRE(max_blocks == 0 || grid_fits(n_segments, 256 / (max_blocks < 256 ? max_blocks : 256)), TF_ESHAPE, "tf_segment_tables: block table too large");
-    TF_REQUIRE(n_segments == 0 || max_blocks == 0 || n_segments < (1ll << 39) / max_blocks, TF_ESHAPE, "tf_segment_tables: block table too large");
+    TF_REQUIRE(n_segments == 0 || max_blocks == 0 || n_segments < (1ll << 38) / max_blocks, TF_ESHAPE, "tf_segment_tables: block table too large");
+    TF_REQUIRE(block_rows < (1ll << 31), TF_ESHAPE, "tf_segment_tables: blocks too large");
     TF_REQUIRE((n_free == 0 || free_blocks) && (n_segments * max_blocks == 0 || block_table), TF_EINVAL, "tf_segment_tables: null block pointer");
-    TF_REQUIRE(workspace_words >= tf_segment_workspace_words(n_segments, block_rows) && (n_segments == 0 || workspace), TF_ESHAPE,
-               "tf_segment_tables: workspace too small");
+    TF_REQUIRE(!slots || index, TF_EINVAL, "tf_segment_tables: slots need an index");
   }
+  TF_REQUIRE(workspace_words >= tf_segment_workspace_words(n_segments, block_rows) && (workspace || !tf_segment_workspace_words(n_segments, block_rows)),
+             TF_ESHAPE, "tf_segment_tables: workspace too small");
   hipStream_t st = (hipStream_t)stream;
-  seg_sums_kernel<<<1, 1024, 0, st>>>((const ll*)lengths, n_segments, n_rows, block_rows, (ll*)offsets, (ll*)workspace);
-  if (blocks && n_segments * max_blocks > 0)
-    seg_blocks_kernel<<<(unsigned)((n_segments * max_blocks + 255) / 256), 256, 0, st>>>((const ll*)lengths, (const ll*)workspace, free_blocks, n_free, n_segments,
-                                                                                       n_rows, block_rows, max_blocks, block_table);
-  if (n_rows > 0 && (index || position || starts || slots))
-    seg_rows_kernel<<<(unsigned)((n_rows + 255) / 256), 256, 0, st>>>((const ll*)offsets, block_table, n_segments, n_rows, block_rows, max_blocks, (ll*)index,
-                                                                    (ll*)position, (ull*)starts, (ll*)slots);
+  const ll cells = blocks ? n_segments * max_blocks : 0;
+  Blocks b = {block_rows, n_free, max_blocks, free_blocks, cells ? block_table : nullptr, (ll*)slots, -1};
+  if (blocks && (block_rows & (block_rows - 1)) == 0)
+    for (b.shift = 0; (1ll << b.shift) < block_rows;) ++b.shift;
+  if (n_segments <= SMALL) {
+    // a workgroup's rows: enough of them to be worth its sums, few enough to fill the card
+    const ll per = n_rows < (1ll << 20) ? 1024 : 8192;
+    ll grid = starts ? (n_rows + per - 1) / per : 0;
+    if (cells && grid < (cells + 1023) / 1024) grid = (cells + 1023) / 1024 < 2048 ? (cells + 1023) / 1024 : 2048;
+    TF_REQUIRE(grid < (1ll << 31), TF_ESHAPE, "tf_segment_tables: too many rows");
+    seg_small_kernel<<<(unsigned)(grid ? grid : 1), 256, 0, st>>>((const ll*)lengths, (int)n_segments, n_rows, per, (ll*)offsets, (ll*)index, (ll*)position,
+                                                                (ull*)starts, b);
+  } else {
+    ll* sums = (ll*)workspace;
+    ll* first = sums + 2 * chunks_of(n_segments);
+    const unsigned grid = (unsigned)chunks_of(n_segments);
+    seg_sums_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ull*)starts, starts ? (n_rows + 63) >> 6 : 0);
+    seg_offsets_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ll*)offsets, first, (ll*)index, (ull*)starts);
+    if (cells) seg_blocks_kernel<<<(unsigned)((cells + 255) / 256), 256, 0, st>>>((const ll*)lengths, first, n_segments, n_rows, b);
+    if (n_rows > 0 && (index || position))
+      seg_rows_kernel<<<(unsigned)((n_rows + 4 * WAVE_ROWS - 1) / (4 * WAVE_ROWS)), 256, 0, st>>>((const ll*)offsets, first, n_segments, n_rows, (const ull*)starts,
+                                                                                              (ll*)index, (ll*)position, b);
+  }
   TF_LAUNCH_CHECK("tf_segment_tables");
   return TF_OK;
 }

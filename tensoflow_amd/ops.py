@@ -546,10 +546,12 @@ def segment_offsets(lengths):
     if lengths.dim() != 1:
         raise RuntimeError(f"lengths must be [R], got {tuple(lengths.shape)}")
     stream = _on(lengths)
-    R, null = lengths.shape[0], C.c_void_p(0)
+    lib, R = L.load(), lengths.shape[0]
     offsets = torch.empty(R + 1, dtype=torch.int64, device=lengths.device)
-    L.check(L.load().tf_segment_tables(_p(lengths, torch.int64, "lengths"), R, _MOST_ROWS, offsets.data_ptr(), null, null, null, 0, null, 0, 0, null, null, null,
-                                       0, stream), "tf_segment_tables")
+    nw = lib.tf_segment_workspace_words(R, 0)
+    work = torch.empty(nw, dtype=torch.int64, device=lengths.device) if nw else None
+    L.check(lib.tf_segment_tables(_p(lengths, torch.int64, "lengths"), R, _MOST_ROWS, offsets.data_ptr(), None, None, None, 0, None, 0, 0, None, None,
+                                  _p(work, torch.int64), nw, stream), "tf_segment_tables")
     return offsets
 
 
@@ -568,20 +570,21 @@ def segment_tables(lengths, n_rows=None, index=True, position=True, block_rows=0
     if n_rows < 0 or block_rows < 0:
         raise RuntimeError("n_rows and block_rows must not be negative")
     new = lambda *s, dtype=torch.int64: torch.empty(s, dtype=dtype, device=dev)
-    t = SegmentTables(n_rows, R, new(R + 1), new(n_rows) if index else None, new(n_rows) if position else None, new((n_rows + 63) // 64))
-    lib, work, n_free = L.load(), None, 0
+    t = SegmentTables(n_rows, R, new(R + 1), new(n_rows) if index or block_rows else None, new(n_rows) if position else None, new((n_rows + 63) // 64))
+    lib, n_free = L.load(), 0
     if block_rows:
         if free_blocks is None:
             free_blocks = torch.arange(n_rows // block_rows + R, dtype=torch.int32, device=dev)
         n_free = free_blocks.numel()
         max_blocks = (n_rows + block_rows - 1) // block_rows if max_blocks is None else max_blocks
         t.block_table, t.slots = new(R, max_blocks, dtype=torch.int32), new(n_rows)
-        work = new(lib.tf_segment_workspace_words(R, block_rows))
     elif free_blocks is not None or max_blocks:
         raise RuntimeError("free_blocks and max_blocks go with block_rows")
+    nw = lib.tf_segment_workspace_words(R, block_rows)
+    work = new(nw) if nw else None
     L.check(lib.tf_segment_tables(pl, R, n_rows, t.offsets.data_ptr(), _p(t.index, torch.int64), _p(t.position, torch.int64), t.starts.data_ptr(),
                                   block_rows, _p(free_blocks, torch.int32, "free_blocks"), n_free, max_blocks or 0, _p(t.block_table, torch.int32),
-                                  _p(t.slots, torch.int64), _p(work, torch.int64), 0 if work is None else work.numel(), stream), "tf_segment_tables")
+                                  _p(t.slots, torch.int64), _p(work, torch.int64), nw, stream), "tf_segment_tables")
     return t
 
 
@@ -705,6 +708,11 @@ def gated_step(state, slots, gate, x, form="decay", out=None):
     if state.dim() < 2 or state.shape[1:].numel() != c:
         raise RuntimeError(f"state must be [S, {c}], got {tuple(state.shape)}")
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    if n > 8192:                                                # what one launch takes
+        for k in range(0, n, 8192):
+            s = slice(k, k + 8192)
+            gated_step(state, slots[s], gate[s], x[s], form, y[s] if out is not None else y[s].zero_())
+        return y
     L.check(L.load().tf_gated_step(C.byref(d), gate.data_ptr(), x.data_ptr(), _p(slots, torch.int64, "slots"), state.shape[0],
                                    _p(state, torch.float32, "state"), _like_x(y, x, "out"), stream), "tf_gated_step")
     return y

@@ -408,6 +408,21 @@ def test_step(dev, b, d, g, t, gt, form):
     assert torch.equal(out[w], y[w]) and bool((out[~w] == 3).all()) and bool((y[~w] == 0).all())
 
 
+def test_step_of_many_rows(dev):
+    """Beyond what one launch takes, a slot's rows in two launches among them."""
+    from tensoflow_amd import ops
+    b, d, S = 9000, 8, 10000
+    gate, x = inputs(b, d, 2, "f32", "f32", "decay", 1)
+    r = torch.Generator().manual_seed(3)
+    pool, slots = torch.randn(S, d, generator=r), torch.randperm(S, generator=r)[:b]
+    slots[8999], slots[5000], slots[8500] = slots[17], -1, slots[8400]
+    state = pool.to(dev)
+    y = ops.gated_step(state, slots.to(dev), gate.to(dev), x.to(dev))
+    want, after, written = rec.step(d64(pool), slots.numpy(), d64(gate), d64(x), "decay")
+    near(y, want, 2.0 ** -24 * 3 * 16 * (1 + np.abs(after).max()) * written[:, None], "y")
+    near(state, after, 2.0 ** -24 * 3 * 16 * (1 + np.abs(after).max()) * (d64(pool) != after), "state")
+
+
 def test_step_after_step_is_the_scan(dev):
     """Ragged prompts through the scan, their end states into the pool, then tokens one by one: the states of the scan over the whole."""
     from tensoflow_amd import ops

@@ -74,7 +74,9 @@ def test_cabi_refusals(lib):
     assert tab(r=-1) == -2 and tab(n=-1) == -2 and tab(br=-1) == -2 and tab(off=None) == -1 and tab(lengths=None) == -1
     assert tab(n=1 << 60) == -2 and b"too many" in err()
     assert tab(bt=a) == -1 and b"without a block size" in err()
-    assert tab(br=4, free=a, nf=2, mb=2, bt=a, sl=a) == -2 and b"workspace" in err()
+    assert tab(r=2049) == -2 and b"workspace" in err() and tab(r=2049, br=4, free=a, nf=2, mb=2, bt=a, sl=a, ws=a, nw=2050) == -2 and b"workspace" in err()
+    assert tab(st=None) == -1 and b"need starts" in err() and tab(br=4, free=a, nf=2, mb=2, bt=a, sl=a, idx=None) == -1 and b"need an index" in err()
+    assert tab(br=1 << 31, free=a, nf=2, mb=2, bt=a, sl=a) == -2 and b"blocks too large" in err()
     assert tab(br=4, free=a, nf=2, mb=1 << 40, bt=a, sl=a, ws=a, nw=2) == -2 and b"too large" in err()
     assert tab(br=4, nf=2, mb=2, bt=a, sl=a, ws=a, nw=2) == -1 and tab(br=4, free=a, nf=2, mb=2, sl=a, ws=a, nw=2) == -1
     assert lib.tf_segment_from_index(a, -1, 2, a, a, None) == -2 and lib.tf_segment_from_index(None, 4, 2, a, a, None) == -1
@@ -92,7 +94,7 @@ def test_cabi_refusals(lib):
     assert lib.tf_gated_scan_fwd(None, a, a, a, a, a, None, a, None, None, a, big, None) == -1 and b"null descriptor" in err()
     # step
     step = lambda d, gate=a, x=a, slots=a, ns=4, state=a, y=a: lib.tf_gated_step(C.byref(d), gate, x, slots, ns, state, y, None)
-    assert step(desc(n_rows=0)) == 0 and step(desc(n_rows=65537)) == -2 and step(desc(), ns=-1) == -2 and step(desc(), slots=None) == -1 and step(desc(), state=None) == -1
+    assert step(desc(n_rows=0)) == 0 and step(desc(n_rows=8193)) == -2 and step(desc(), ns=-1) == -2 and step(desc(), slots=None) == -1 and step(desc(), state=None) == -1
     assert step(desc(), y=None) == -1 and step(desc(form=-1)) == -1
 
 
