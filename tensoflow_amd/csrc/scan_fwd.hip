@@ -1,0 +1,148 @@
+// Forward pass of the gated linear recurrence over a packed batch (scan_tile.h has the decomposition).
+//   TF_GATE_DECAY: a = g, b = x;   TF_GATE_LOG: a = exp(g), b = x;   TF_GATE_ALPHA: a = 1 - g, b = g x (compositing).
+#include "scan_tile.h"
+
+using namespace tfscan;
+
+namespace {
+
+template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
+__global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __restrict__ y, float* __restrict__ final, float* __restrict__ carry) {
+  extern __shared__ __attribute__((aligned(16))) float smem[];
+  __shared__ unsigned s_ticket;
+  __shared__ int s_closed[8], s_opened;
+  constexpr int AV = SHARED ? 1 : V;
+  const int nw = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  float *sA = smem, *sB = smem + nw * p.W;
+  char* buf = reinterpret_cast<char*>(smem + (2 * nw * p.W + 3 & ~3)) + wave * p.narrow;
+  const ll lo = max(p.offsets[0], 0ll), hi = min(p.offsets[p.n_seg], p.n_rows);
+  int slab;
+  const int q = take_job(p, &s_ticket, slab);
+  if (slab < 0) {
+    empty_segments(p, (ll)q * nw + wave, p.h0, final);
+    return;
+  }
+  const int cl = WIDE ? lane : lane & (p.CL - 1), rl = WIDE ? 0 : lane / p.CL, RL = WIDE ? 1 : 64 / p.CL, T = nw * RL * K;
+  const Lane<V, SHARED> l(p, slab, cl);
+  const Rows<WIDE> r(p, (ll)q * T + (wave * RL + rl) * K, T, lo, hi);
+  const ll t0 = (ll)(p.reverse ? p.tiles - 1 - q : q) * T;  // the tile's lowest row, and its wave's
+  const ll w0 = t0 + (ll)(p.reverse ? nw - 1 - wave : wave) * RL * K;
+  const int block = p.reverse ? RL - 1 - rl : rl;
+  const bool full = t0 >= lo && t0 + T <= hi, turned = !WIDE && p.narrow && full;
+  Vec<XT, V> rx[K];
+  Vec<GT, AV> rg[K];
+  unsigned first, last;
+  if (turned) {
+    Turn<XT, V> tx(p.D, RL);
+    Turn<GT, AV> tg(p.G, RL);
+    tx.load(static_cast<const XT*>(p.x) + w0 * p.D);
+    tg.load(static_cast<const GT*>(p.gate) + w0 * p.G);
+    r.bits(p, hi, first, last);
+    tx.to_rows(buf, p.D, block, l.c, p.reverse, rx);
+    tg.to_rows(buf, p.G, block, l.g, p.reverse, rg);
+  } else {
+    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, p.aligned && full, rx);
+    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, p.aligned && full, rg);
+    r.bits(p, hi, first, last);
+  }
+  float a[K][AV], b[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[k][v] = to_f(rx[k].v[v]);
+#pragma unroll
+    for (int v = 0; v < AV; ++v) a[k][v] = to_f(rg[k].v[v]);
+  }
+  if (p.form == TF_GATE_LOG) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int v = 0; v < AV; ++v) a[k][v] = exp_gate(a[k][v]);
+  } else if (p.form == TF_GATE_ALPHA) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) b[k][v] *= a[k][AV == 1 ? 0 : v];
+#pragma unroll
+      for (int v = 0; v < AV; ++v) a[k][v] = 1.f - a[k][v];
+    }
+  }
+  // a first row begins from h0 (or 0), a row of no segment from 0: it holds b = 0 and leaves 0
+  unsigned cut = first | (~r.valid & ((1u << K) - 1));
+  float A[AV], B[V], eA[AV], eB[V];
+  bool closed = cut != 0, eclosed;
+#pragma unroll
+  for (int v = 0; v < AV; ++v) A[v] = 1.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) B[v] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    cut_at<V, WIDE>(p, k, cut, first, p.h0, r.p0 + k * r.step, l.c, B);
+#pragma unroll
+    for (int v = 0; v < V; ++v) B[v] = fmaf(a[k][AV == 1 ? 0 : v], B[v], b[k][v]);
+#pragma unroll
+    for (int v = 0; v < AV; ++v) A[v] *= a[k][v];
+  }
+  if (!WIDE) wave_join<V, AV, false>(p, A, B, closed, eA, eB, eclosed);
+  if (rl == RL - 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      sA[wave * p.W + cl * V + v] = A[AV == 1 ? 0 : v];
+      sB[wave * p.W + cl * V + v] = B[v];
+    }
+    if (cl == 0) s_closed[wave] = closed;
+  }
+  if (threadIdx.x == 0) s_opened = cut & 1;
+  __syncthreads();
+  join_waves<V, SHARED, false>(p, q, slab, nw, sA, sB, s_closed, s_opened, carry);
+  __syncthreads();
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float s = sB[wave * p.W + cl * V + v];
+    h[v] = WIDE ? s : eclosed ? eB[v] : fmaf(eA[AV == 1 ? 0 : v], s, eB[v]);
+  }
+  const Turn<XT, V> ty(p.D, RL);
+  cut = again<WIDE>(cut);
+  first = again<WIDE>(first);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const ll at = r.p0 + k * r.step;
+    cut_at<V, WIDE>(p, k, cut, first, p.h0, at, l.c, h);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][AV == 1 ? 0 : v], h[v], b[k][v]);
+    if (l.ok) {
+      if (turned) ty.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(h));
+      else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h, p.aligned);
+      if (final && (last >> k & 1)) put_state<V>(p, final, at, l.c, h);
+    }
+  }
+  if (turned) ty.store(buf, y + w0 * p.D);
+}
+
+template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
+void launch_fwd(const Launch& L, void* y, float* final, float* carry) {
+  scan_fwd_kernel<XT, GT, V, SHARED, WIDE><<<L.blocks, L.g.nw * 64, L.lds, L.stream>>>(L.a, static_cast<XT*>(y), final, carry);
+}
+
+}  // namespace
+
+extern "C" int tf_gated_scan_fwd(const TfGatedScan* d, const void* gate, const void* x, const int64_t* offsets, const int64_t* index, const uint64_t* starts,
+                                 const float* h0, void* y, float* final, float* carry, float* workspace, size_t workspace_floats, tf_stream_t stream) {
+  if (int rc = check_desc(d, "tf_gated_scan_fwd")) return rc;
+  TF_REQUIRE(offsets && (d->n_rows == 0 || (gate && x && y && starts)), TF_EINVAL, "tf_gated_scan_fwd: null pointer");
+  TF_REQUIRE(d->n_rows == 0 || index || (!h0 && !final), TF_EINVAL, "tf_gated_scan_fwd: h0 and final need an index");
+  const size_t need = tf_gated_scan_workspace_floats(d, 0);
+  TF_REQUIRE(workspace_floats >= need && (!need || (workspace && ((size_t)workspace & 7) == 0)), TF_ESHAPE,
+             "tf_gated_scan_fwd: workspace too small, or not aligned to 8 bytes");
+  Launch L;
+  const void* like_x[2] = {y, nullptr};
+  if (int rc = prepare(*d, "tf_gated_scan_fwd", gate, x, offsets, index, starts, h0, final != nullptr, workspace, stream, like_x, nullptr, 2, &L)) return rc;
+  if (L.blocks) {
+#define CALL(XT, GT, V, SH, WIDE) launch_fwd<XT, GT, V, SH, WIDE>(L, y, final, carry)
+    TF_SCAN_DISPATCH(CALL, *d)
+#undef CALL
+  }
+  TF_LAUNCH_CHECK("tf_gated_scan_fwd");
+  return TF_OK;
+}
