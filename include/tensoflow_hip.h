@@ -224,7 +224,9 @@ typedef enum TfGateForm {
 } TfGateForm;
 
 /* x [n_rows, channels] and gate [n_rows, gates] with row strides in elements; one gate serves channels / gates consecutive channels.
- * x is fp32, fp16 or bf16, the gate of the same type or fp32; states are fp32, y and the gradients are rounded once to their inputs' types. */
+ * x is fp32, fp16 or bf16, the gate of the same type or fp32; states are fp32, y and the gradients are rounded once to their inputs' types.
+ * The scan reads V elements at once, V the largest of 4, 3, 2, 1 that divides the channels of a gate (all channels, where each has its own):
+ * for V = 2 and 4 rows of x, y and their gradients (and of a gate for each channel) have to be aligned to V elements. */
 typedef struct TfGatedScan {
   int64_t n_rows, n_segments;
   int64_t ld_x, ld_gate;

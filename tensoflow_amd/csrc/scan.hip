@@ -115,7 +115,8 @@ int prepare(const TfGatedScan& d, const char* who, const void* gate, const void*
   auto all = [&](size_t bx, size_t bg) {
     return fits(x, bx) && fits(like_x[0], bx) && fits(like_x[1], bx) && fits(gate, bg) && fits(like_gate, bg);
   };
-  a.aligned = all(vx * xs, vg * gs) && d.ld_x % vx == 0 && d.ld_gate % vg == 0;
+  TF_REQUIRE(all(vx * xs, vg * gs) && (d.n_rows <= 1 || (d.ld_x % vx == 0 && d.ld_gate % vg == 0)), TF_EINVAL,
+             "%s: rows of x must be aligned to %d elements, of the gate to %d", who, vx, vg);
   const size_t join = ((size_t)g.nw * g.W * lds_floats + 3) / 4 * 16;
   // rows shorter than a cache line, side by side in memory: turned in LDS
   if (g.slabs == 1 && d.channels * xs < 128 && all(16, 16) && d.ld_x == d.channels && d.ld_gate == d.gates) {
@@ -147,7 +148,7 @@ namespace {
 
 // A workgroup is a row and 256 V of its channels.  The first row of a slot takes the later ones of the same slot along, in order; the others leave.
 template <typename XT, typename GT, int V, bool SHARED>
-__global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, const GT* __restrict__ gate, const XT* __restrict__ x, const ll* __restrict__ slots,
+__global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, const GT* __restrict__ gate, const XT* __restrict__ x, const ll* __restrict__ slots,
                                                    ll n_slots, float* __restrict__ state, XT* __restrict__ y) {
   constexpr int AV = SHARED ? 1 : V;
   const int D = d.channels, P = D / d.gates, n = (int)d.n_rows, r = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * V;
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, c
   const ll slot = slots[r];
   if (slot < 0 || slot >= n_slots) {
     const float z[V] = {};
-    if (d.zero_rest && mine) store_v<XT, V>(y + (ll)r * D + c, z, aligned);
+    if (d.zero_rest && mine) store_v<XT, V>(y + (ll)r * D + c, z);
     return;
   }
   const ll g = SHARED ? c / P : c;
@@ -163,9 +164,9 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, c
   Vec<GT, AV> rg;
   Vec<float, V> h;
   if (mine) {  // asked for before the search, which needs none of it
-    rx = load_v<XT, V>(x + r * d.ld_x + c, aligned);
-    rg = load_v<GT, AV>(gate + r * d.ld_gate + g, aligned);
-    h = load_v<float, V>(state + slot * D + c, aligned);
+    rx = load_v<XT, V>(x + r * d.ld_x + c);
+    rg = load_v<GT, AV>(gate + r * d.ld_gate + g);
+    h = load_v<float, V>(state + slot * D + c);
   }
   int last = r;
   if (n > 1) {
@@ -182,8 +183,8 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, c
   for (int q = r; q <= last; ++q) {
     if (q != r) {
       if (slots[q] != slot) continue;
-      rx = load_v<XT, V>(x + q * d.ld_x + c, aligned);
-      rg = load_v<GT, AV>(gate + q * d.ld_gate + g, aligned);
+      rx = load_v<XT, V>(x + q * d.ld_x + c);
+      rg = load_v<GT, AV>(gate + q * d.ld_gate + g);
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -192,9 +193,9 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, int aligned, c
       if (d.form == TF_GATE_ALPHA) b *= a, a = 1.f - a;
       h.v[v] = fmaf(a, h.v[v], b);
     }
-    store_v<XT, V>(y + (ll)q * D + c, h.v, aligned);
+    store_v<XT, V>(y + (ll)q * D + c, h.v);
   }
-  store_v<float, V>(state + slot * D + c, h.v, aligned);
+  store_v<float, V>(state + slot * D + c, h.v);
 }
 
 }  // namespace
@@ -218,13 +219,13 @@ extern "C" int tf_gated_step(const TfGatedScan* d, const void* gate, const void*
   // four channels a lane, unless that leaves most of the card idle: one row of 2048 channels is 8 workgroups at one channel a lane
   const bool shared = d->channels != d->gates;
   const int unit = shared ? d->channels / d->gates : d->channels;
-  const int V = unit % 4 == 0 && d->n_rows * d->channels >= 65536 ? 4 : 1;
   const size_t xs = d->x_type == TF_TYPE_F32 ? 4 : 2, gs = d->gate_type == TF_TYPE_F32 ? 4 : 2;
-  const int vg = shared ? 1 : V;
-  const int aligned = fits(x, V * xs) && fits(y, V * xs) && fits(gate, vg * gs) && fits(state, V * 4) && (d->n_rows == 1 || (d->ld_x % V == 0 && d->ld_gate % vg == 0));
+  const int vg = shared ? 1 : 4;
+  const bool aligned = fits(x, 4 * xs) && fits(y, 4 * xs) && fits(gate, vg * gs) && fits(state, 16) && (d->n_rows == 1 || (d->ld_x % 4 == 0 && d->ld_gate % vg == 0));
+  const int V = unit % 4 == 0 && aligned && d->n_rows * d->channels >= 65536 ? 4 : 1;
   const dim3 grid((unsigned)((d->channels + 256 * V - 1) / (256 * V)), (unsigned)d->n_rows);
   hipStream_t st = (hipStream_t)stream;
-#define STEP(XT, GT, VV, SH) step_kernel<XT, GT, VV, SH><<<grid, 256, 0, st>>>(*d, aligned, static_cast<const GT*>(gate), static_cast<const XT*>(x), (const ll*)slots, n_slots, state, static_cast<XT*>(y))
+#define STEP(XT, GT, VV, SH) step_kernel<XT, GT, VV, SH><<<grid, 256, 0, st>>>(*d, static_cast<const GT*>(gate), static_cast<const XT*>(x), (const ll*)slots, n_slots, state, static_cast<XT*>(y))
 #define STEP_V(XT, GT)                                                            \
   if (V == 4) { if (shared) STEP(XT, GT, 4, true); else STEP(XT, GT, 4, false); } \
   else { if (shared) STEP(XT, GT, 1, true); else STEP(XT, GT, 1, false); }

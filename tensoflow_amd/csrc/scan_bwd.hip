@@ -78,9 +78,9 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
     tg.to_rows(buf, p.G, block, l.g, p.reverse, rg);
     if (gy) ty.to_rows(buf, p.D, block, l.c, p.reverse, ry);
   } else {
-    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, p.aligned && full, rx);
-    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, p.aligned && full, rg);
-    if (gy) direct_rows<XT, V, WIDE>(p, gy, p.D, r, l.c, p.aligned && full, ry);
+    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, rx);
+    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, rg);
+    if (gy) direct_rows<XT, V, WIDE>(p, gy, p.D, r, l.c, full, ry);
     r.bits(p, hi, first, last);
   }
   // ga: a, or g itself where a = 1 - g; a = ga * s1 + s0, exact where nothing is to be done
@@ -96,7 +96,11 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
       g[k][v] = gy ? to_f(ry[k].v[v]) : 0.f;
     }
 #pragma unroll
-    for (int v = 0; v < AV; ++v) ga[k][v] = logs ? exp_gate(to_f(rg[k].v[v])) : to_f(rg[k].v[v]);
+    for (int v = 0; v < AV; ++v) ga[k][v] = to_f(rg[k].v[v]);
+    if (logs) {
+#pragma unroll
+      for (int v = 0; v < AV; ++v) ga[k][v] = exp_gate(ga[k][v]);
+    }
   }
   const unsigned none = ~r.valid & ((1u << K) - 1);
   unsigned cut = first | none, mcut = last | none;
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
     }
     if (dx && l.ok) {
       if (turned) tx.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(o));
-      else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((dx + at * p.D) + l.c, o, p.aligned);
+      else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((dx + at * p.D) + l.c, o);
     }
     if (dh0 && l.ok && (first >> k & 1)) put_state<V>(p, dh0, at, l.c, m);
   }
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
     }
     if (!SHARED) {
       og[k] = round_v<GT, AV>(d);
-      if (!turned && l.ok && (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1)))) store_v<GT, AV>(dgate + at * p.G + l.g, d, p.aligned);
+      if (!turned && l.ok && (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1)))) store_v<GT, AV>(dgate + at * p.G + l.g, d);
     } else {
       sums[k] = 0.f;
 #pragma unroll

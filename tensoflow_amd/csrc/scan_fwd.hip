@@ -41,8 +41,8 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
     tx.to_rows(buf, p.D, block, l.c, p.reverse, rx);
     tg.to_rows(buf, p.G, block, l.g, p.reverse, rg);
   } else {
-    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, p.aligned && full, rx);
-    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, p.aligned && full, rg);
+    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, rx);
+    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, rg);
     r.bits(p, hi, first, last);
   }
   float a[K][AV], b[K][V];
@@ -52,15 +52,10 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
     for (int v = 0; v < V; ++v) b[k][v] = to_f(rx[k].v[v]);
 #pragma unroll
     for (int v = 0; v < AV; ++v) a[k][v] = to_f(rg[k].v[v]);
-  }
-  if (p.form == TF_GATE_LOG) {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    if (p.form == TF_GATE_LOG) {
 #pragma unroll
       for (int v = 0; v < AV; ++v) a[k][v] = exp_gate(a[k][v]);
-  } else if (p.form == TF_GATE_ALPHA) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
+    } else if (p.form == TF_GATE_ALPHA) {
 #pragma unroll
       for (int v = 0; v < V; ++v) b[k][v] *= a[k][AV == 1 ? 0 : v];
 #pragma unroll
@@ -113,7 +108,7 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
     for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][AV == 1 ? 0 : v], h[v], b[k][v]);
     if (l.ok) {
       if (turned) ty.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(h));
-      else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h, p.aligned);
+      else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h);
       if (final && (last >> k & 1)) put_state<V>(p, final, at, l.c, h);
     }
   }

@@ -29,7 +29,7 @@ struct ScanArgs {
   const ull* starts;
   const float* h0;
   ll n_rows, n_seg, ld_x, ld_gate;
-  int tiles, D, G, P, form, reverse, zero_rest, aligned;
+  int tiles, D, G, P, form, reverse, zero_rest;
   int CL, W, LP, hs, parts, slabs;  // lanes across channels, channels of a workgroup; lanes of a head, heads of a workgroup, workgroups of a head
   int narrow;                       // bytes of a wave's buffer where rows are shorter than a cache line, or 0
   int tickets;                      // distance between the counters of the slabs
@@ -86,14 +86,37 @@ template <typename T, int V>
 struct alignas((V & (V - 1)) ? sizeof(T) : sizeof(T) * V) Vec {
   T v[V];
 };
+// Stored as whole words: the compiler takes a vector of 16-bit values apart into stores of single ones (65536 x 1024 bf16: 1.17 million store
+// instructions in place of 0.29), unless their words are beyond its sight.
 template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_v(const T* p, bool aligned) {
-  if (aligned) return *reinterpret_cast<const Vec<T, V>*>(p);
-  Vec<T, V> r;
+__device__ __forceinline__ void put_words(void* p, const Vec<T, V>& r) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES % 4 == 0) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    constexpr int N = BYTES / 4;
+    unsigned w[N];
 #pragma unroll
-  for (int v = 0; v < V; ++v) r.v[v] = p[v];
-  return r;
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __builtin_bit_cast(unsigned, r.v[i]);
+      } else {
+        w[i] = __builtin_bit_cast(unsigned short, r.v[2 * i]) | (unsigned)__builtin_bit_cast(unsigned short, r.v[2 * i + 1]) << 16;
+        asm("" : "+v"(w[i]));
+      }
+    }
+    if constexpr (N == 4) *static_cast<u4*>(p) = u4{w[0], w[1], w[2], w[3]};
+    else if constexpr (N == 2) *static_cast<u2*>(p) = u2{w[0], w[1]};
+    else
+#pragma unroll
+      for (int i = 0; i < N; ++i) static_cast<unsigned*>(p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) static_cast<T*>(p)[v] = r.v[v];
+  }
 }
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_v(const T* p) { return *reinterpret_cast<const Vec<T, V>*>(p); }
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> round_v(const float* f) {
   Vec<T, V> r;
@@ -102,15 +125,7 @@ __device__ __forceinline__ Vec<T, V> round_v(const float* f) {
   return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float* f, bool aligned) {
-  const Vec<T, V> r = round_v<T, V>(f);
-  if (aligned) {
-    *reinterpret_cast<Vec<T, V>*>(p) = r;
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = r.v[v];
-  }
-}
+__device__ __forceinline__ void store_v(T* p, const float* f) { put_words<T, V>(p, round_v<T, V>(f)); }
 
 __device__ __forceinline__ unsigned clean(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 // exp(g) = 2^(g log2 e) on the hardware's 2^x (1 ulp): g's product is rounded once, a relative error of the result of |g| 2^-24
@@ -333,7 +348,7 @@ struct Turn {
   }
   // and back: the lane's row k
   __device__ __forceinline__ void put(char* buf, int width, int block, int c, bool reverse, int k, const Vec<T, V>& v) const {
-    *reinterpret_cast<Vec<T, V>*>(reinterpret_cast<T*>(buf + block * (unit + 1) * 16) + (reverse ? K - 1 - k : k) * width + c) = v;
+    put_words<T, V>(reinterpret_cast<T*>(buf + block * (unit + 1) * 16) + (reverse ? K - 1 - k : k) * width + c, v);
   }
   __device__ __forceinline__ void store(const char* buf, T* rows) const {
     const int lane = threadIdx.x & 63;
@@ -346,19 +361,19 @@ struct Turn {
 
 // the lane's rows as they lie in memory
 template <typename T, int V, bool WIDE>
-__device__ __forceinline__ void direct_rows(const ScanArgs& p, const T* base, ll ld, const Rows<WIDE>& r, int c, bool fast, Vec<T, V> (&out)[K]) {
-  if (fast) {
+__device__ __forceinline__ void direct_rows(const ScanArgs& p, const T* base, ll ld, const Rows<WIDE>& r, int c, bool full, Vec<T, V> (&out)[K]) {
+  if (full) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const T* row = base + (r.p0 + k * r.step) * ld;
-      out[k] = load_v<T, V>(row + c, true);
+      out[k] = load_v<T, V>(row + c);
     }
   } else {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const T* row = base + (r.p0 + k * r.step) * ld;
       if (r.valid >> k & 1) {
-        out[k] = load_v<T, V>(row + c, false);
+        out[k] = load_v<T, V>(row + c);
       } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) out[k].v[v] = from_f<T>(0.f);

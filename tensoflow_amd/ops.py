@@ -634,6 +634,25 @@ def _scan_desc(gate, x, n_segments, form, reverse, zero_rest):
     return L.TfGatedScan(n, n_segments, ldx, ldg, c, g, _TYPES[x.dtype], _TYPES[gate.dtype], _GATE_FORMS[form], 1 if reverse else 0, zero_rest), n, c
 
 
+def _aligned(t, d, shared):
+    """t with rows aligned to what the scan reads at once (a copy where they are not: a column slice at an odd place)."""
+    unit = d.channels // d.gates if shared else d.channels
+    v = 4 if unit % 4 == 0 else 1 if unit % 3 == 0 else 2 if unit % 2 == 0 else 1
+    if v > 1 and (t.data_ptr() % (v * t.element_size()) or (t.shape[0] > 1 and t.stride(0) % v)):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _scan_inputs(gate, x, d):
+    shared = d.gates != d.channels
+    x = _aligned(x, d, shared)
+    d.ld_x = x.stride(0)
+    if not shared:
+        gate = _aligned(gate, d, False)
+        d.ld_gate = gate.stride(0)
+    return gate, x
+
+
 def _like_x(t, x, name):
     if t.shape != x.shape or t.dtype != x.dtype:
         raise RuntimeError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
@@ -659,9 +678,12 @@ def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final
         raise RuntimeError(f"x has {n} rows, the tables {tables.n_rows}")
     if tables.index is None and (h0 is not None or want_final):
         raise RuntimeError("h0 and final need tables with an index")
+    gate, x = _scan_inputs(gate, x, d)
     ph = _state(h0, R, c, "h0")
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    py = _like_x(y, x, "out")
+    _like_x(y, x, "out")
+    y = _aligned(y, d, d.gates != d.channels)
+    py = _p(y, x.dtype, "out")
     new = lambda k: torch.empty(k, dtype=torch.float32, device=x.device) if k else None
     final = torch.empty(R, *x.shape[1:], dtype=torch.float32, device=x.device) if want_final else None
     lib = L.load()
@@ -670,6 +692,8 @@ def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final
     work = new(nw)
     L.check(lib.tf_gated_scan_fwd(C.byref(d), gate.data_ptr(), x.data_ptr(), tables.offsets.data_ptr(), _p(tables.index, torch.int64), tables.starts.data_ptr(),
                                   ph, py, _p(final), _p(carry), _p(work), nw, stream), "tf_gated_scan_fwd")
+    if out is not None and y is not out:
+        y = out.copy_(y)
     return (y, final, carry) if want_carry else (y, final)
 
 
@@ -683,6 +707,8 @@ def gated_scan_bwd(gate, x, tables, carry, gy, g_final, h0=None, form="decay", r
     if tables.index is None and (h0 is not None or g_final is not None or need_h0):
         raise RuntimeError("h0 and final need tables with an index")
     lib = L.load()
+    gate, x = _scan_inputs(gate, x, d)
+    gy = None if gy is None else _aligned(gy, d, d.gates != d.channels)
     if carry.numel() != lib.tf_gated_scan_carry_floats(C.byref(d)):
         raise RuntimeError("carry is not of this scan")
     ph, pf = _state(h0, R, c, "h0"), _state(g_final, R, c, "g_final")

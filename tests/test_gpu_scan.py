@@ -272,6 +272,9 @@ def test_scan_strides_and_alignment(dev, t, off):
         plain = ops.gated_scan_bwd(gate.to(dev), x.to(dev), tab, carry, gy.clone(), None)
         for p, q in zip(plain, ops.gated_scan_bwd(gs, xs, tab, carry, gy, None)):
             assert torch.equal(p, q)
+        room = torch.full((n * d + 7 + off,), 3.0, dtype=x.dtype, device=dev)
+        o, _ = ops.gated_scan(gs, xs, tab, out=room[off:off + n * d].view(n, d))
+        assert torch.equal(o, a) and torch.equal(room[off:off + n * d].view(n, d), a) and bool((room[off + n * d:] == 3).all()) and bool((room[:off] == 3).all())
         c, _ = ops.gated_scan(gate.to(dev).view(n, g), x.to(dev).view(n, g, d // g), tab)
         assert c.shape == (n, g, d // g) and torch.equal(c.view(n, d), a)
         row = gate[:1].to(dev).expand(n, g)

@@ -89,8 +89,9 @@ def test_cabi_refusals(lib):
         assert run(desc(n_rows=-1)) == -2 and run(desc(n_segments=-1)) == -2 and run(desc(channels=0)) == -2 and run(desc(gates=3)) == -2 and run(desc(gates=0)) == -2
         assert run(desc(channels=1 << 20, gates=1)) == -2 and run(desc(ld_x=-4)) == -2 and run(desc(n_rows=1 << 40)) == -2
         assert run(desc(x_type=3)) == -1 and run(desc(x_type=0, gate_type=1)) == -1 and run(desc(x_type=1, gate_type=2)) == -1 and run(desc(form=3)) == -1
+        assert run(desc(n_rows=100, ld_x=5)) == -1 and run(desc(), x=a + 4) == -1 and b"aligned" in err() and run(desc(gates=4, ld_gate=5)) == -1
         assert run(desc(), gate=None) == -1 and run(desc(), x=None) == -1 and run(desc(), off=None) == -1
-    assert fwd(desc(), y=None) == -1
+    assert fwd(desc(), y=None) == -1 and fwd(desc(), y=a + 4) == -1 and fwd(desc(n_rows=100000), nw=0) == -2 and b"workspace" in err()
     assert lib.tf_gated_scan_fwd(None, a, a, a, a, a, None, a, None, None, a, big, None) == -1 and b"null descriptor" in err()
     # step
     step = lambda d, gate=a, x=a, slots=a, ns=4, state=a, y=a: lib.tf_gated_step(C.byref(d), gate, x, slots, ns, state, y, None)
