@@ -38,8 +38,9 @@ Geo geometry(const TfGatedScan& d) {
   g.W = g.CL * g.V;
   const ll wave_rows = (64 / g.CL) * K;
   // waves of a workgroup: as many as leave two workgroups to every CU, or as hold all rows in one tile
-  // (four at most where rows are shorter than a cache line: their buffers take 9 KB of LDS a wave)
-  const int most = D * (d.x_type == TF_TYPE_F32 ? 4 : 2) < 128 ? 4 : 8;
+  // (four at most where rows are shorter than a cache line: their buffers take 9 KB of LDS a wave; and for fp32, whose kernels' registers leave room
+  // for 12 waves on a CU: three workgroups of four, where eight waves would be alone)
+  const int most = d.x_type == TF_TYPE_F32 || D < 64 ? 4 : 8;
   g.nw = most;
   while (g.nw > 1 && ((d.n_rows + g.nw * wave_rows - 1) / (g.nw * wave_rows)) * g.slabs < 512) g.nw >>= 1;
   for (int w = 1; w <= most; w <<= 1)
@@ -160,13 +161,15 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, const GT* __re
     return;
   }
   const ll g = SHARED ? c / P : c;
-  Vec<XT, V> rx;
-  Vec<GT, AV> rg;
-  Vec<float, V> h;
+  Raw<XT, V> rx;
+  Raw<GT, AV> rg;
+  float h[V];
   if (mine) {  // asked for before the search, which needs none of it
     rx = load_v<XT, V>(x + r * d.ld_x + c);
     rg = load_v<GT, AV>(gate + r * d.ld_gate + g);
-    h = load_v<float, V>(state + slot * D + c);
+    const Raw<float, V> s = load_v<float, V>(state + slot * D + c);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = s[v];
   }
   int last = r;
   if (n > 1) {
@@ -188,14 +191,14 @@ __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, const GT* __re
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a = to_f(rg.v[AV == 1 ? 0 : v]), b = to_f(rx.v[v]);
+      float a = rg[AV == 1 ? 0 : v], b = rx[v];
       if (d.form == TF_GATE_LOG) a = exp_gate(a);
       if (d.form == TF_GATE_ALPHA) b *= a, a = 1.f - a;
-      h.v[v] = fmaf(a, h.v[v], b);
+      h[v] = fmaf(a, h[v], b);
     }
-    store_v<XT, V>(y + (ll)q * D + c, h.v);
+    store_v<XT, V>(y + (ll)q * D + c, h);
   }
-  store_v<float, V>(state + slot * D + c, h.v);
+  store_v<float, V>(state + slot * D + c, h);
 }
 
 }  // namespace

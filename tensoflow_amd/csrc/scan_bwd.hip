@@ -9,12 +9,9 @@ using namespace tfscan;
 
 namespace {
 
-#ifndef BWD_WAVES
-#define BWD_WAVES 2
-#endif
 
-// sums over LP lanes of K values -> the first lane of the head has out[k].  LP = 2^n: halves of the values change sides (K - 1 shuffles and one for
-// each further doubling, in place of K for each), and lane i of the first K has the value of row i: `mine`.
+// sums over the LP lanes of a head of K values: the first lane has them all
+template <int K>
 __device__ __forceinline__ void head_sums(float (&s)[K], int wl, int LP) {
   for (int o = 1; o < LP; o <<= 1) {
 #pragma unroll
@@ -24,6 +21,9 @@ __device__ __forceinline__ void head_sums(float (&s)[K], int wl, int LP) {
     }
   }
 }
+// LP = 2^n >= K: halves of the values change sides, so that K - 1 shuffles do what K for each doubling did, and one for each further doubling; lane wl has the
+// sum of the row that has wl's low bits in reversed order
+template <int K>
 __device__ __forceinline__ float head_sums_pow2(float (&s)[K], int wl, int LP) {
 #pragma unroll
   for (int n = K / 2, o = 1; n >= 1; n >>= 1, o <<= 1) {
@@ -37,11 +37,12 @@ __device__ __forceinline__ float head_sums_pow2(float (&s)[K], int wl, int LP) {
   }
   float v = s[0];
   for (int o = K; o < LP; o <<= 1) v += __shfl_xor(v, o);
-  return v;  // of row K/2 (wl & 1) + K/4 (wl >> 1 & 1) + ...
+  return v;
 }
 
+// Packed 16-bit values leave room for two workgroups on a CU (16385 x 2048 bf16 with 16 gates: 119 -> 88 us); fp32 ones do not, and are not squeezed.
 template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
-__global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, const float* __restrict__ carry, const XT* __restrict__ gy, const float* __restrict__ gfinal,
+__global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const float* __restrict__ carry, const XT* __restrict__ gy, const float* __restrict__ gfinal,
                                                        GT* __restrict__ dgate, float* __restrict__ dgate_parts, XT* __restrict__ dx, float* __restrict__ dh0) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
   __shared__ unsigned s_ticket;
@@ -64,8 +65,8 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
   const ll w0 = t0 + (ll)(p.reverse ? nw - 1 - wave : wave) * RL * K;
   const int block = p.reverse ? RL - 1 - rl : rl;
   const bool full = t0 >= lo && t0 + T <= hi, turned = !WIDE && p.narrow && full;
-  Vec<XT, V> rx[K], ry[K];
-  Vec<GT, AV> rg[K];
+  Raw<XT, V> x[K], ry[K];
+  Raw<GT, AV> g[K];
   unsigned first, last;
   if (turned) {
     Turn<XT, V> tx(p.D, RL), ty(p.D, RL);
@@ -74,34 +75,24 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
     tg.load(static_cast<const GT*>(p.gate) + w0 * p.G);
     if (gy) ty.load(gy + w0 * p.D);
     r.bits(p, hi, first, last);
-    tx.to_rows(buf, p.D, block, l.c, p.reverse, rx);
-    tg.to_rows(buf, p.G, block, l.g, p.reverse, rg);
+    tx.to_rows(buf, p.D, block, l.c, p.reverse, x);
+    tg.to_rows(buf, p.G, block, l.g, p.reverse, g);
     if (gy) ty.to_rows(buf, p.D, block, l.c, p.reverse, ry);
   } else {
-    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, rx);
-    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, rg);
-    if (gy) direct_rows<XT, V, WIDE>(p, gy, p.D, r, l.c, full, ry);
+    direct_rows<XT, V, WIDE>(static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, x);
+    direct_rows<GT, AV, WIDE>(static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, g);
+    if (gy) direct_rows<XT, V, WIDE>(gy, p.D, r, l.c, full, ry);
     r.bits(p, hi, first, last);
   }
-  // ga: a, or g itself where a = 1 - g; a = ga * s1 + s0, exact where nothing is to be done
+  if (!gy) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) ry[k].zero();
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) gates_kept<GT, AV>(g[k], p.form);
   bool alpha = p.form == TF_GATE_ALPHA;
   const bool logs = p.form == TF_GATE_LOG;
-  float s1 = alpha ? -1.f : 1.f, s0 = alpha ? 1.f : 0.f;
-  float ga[K][AV], x[K][V], g[K][V];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      x[k][v] = to_f(rx[k].v[v]);
-      g[k][v] = gy ? to_f(ry[k].v[v]) : 0.f;
-    }
-#pragma unroll
-    for (int v = 0; v < AV; ++v) ga[k][v] = to_f(rg[k].v[v]);
-    if (logs) {
-#pragma unroll
-      for (int v = 0; v < AV; ++v) ga[k][v] = exp_gate(ga[k][v]);
-    }
-  }
+  const float s1 = alpha ? -1.f : 1.f, s0 = alpha ? 1.f : 0.f;
   const unsigned none = ~r.valid & ((1u << K) - 1);
   unsigned cut = first | none, mcut = last | none;
   float A[AV], B[V], eA[AV], eB[V], P[AV], Q[V], eP[AV], eQ[V];
@@ -113,21 +104,25 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     cut_at<V, WIDE>(p, k, cut, first, p.h0, r.p0 + k * r.step, l.c, B);
+    float ga[AV];
+    gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float gav = ga[k][AV == 1 ? 0 : v];
+      const float gav = ga[AV == 1 ? 0 : v];
       B[v] = fmaf(fmaf(gav, s1, s0), B[v], alpha ? gav * x[k][v] : x[k][v]);
     }
 #pragma unroll
-    for (int v = 0; v < AV; ++v) A[v] *= fmaf(ga[k][v], s1, s0);
+    for (int v = 0; v < AV; ++v) A[v] *= fmaf(ga[v], s1, s0);
   }
 #pragma unroll
   for (int v = 0; v < AV; ++v) P[v] = A[v];
 #pragma unroll
   for (int k = K - 1; k >= 0; --k) {
     cut_at<V, WIDE>(p, k, mcut, last, gfinal, r.p0 + k * r.step, l.c, Q);
+    float ga[AV];
+    gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
-    for (int v = 0; v < V; ++v) Q[v] = fmaf(ga[k][AV == 1 ? 0 : v], s1, s0) * (g[k][v] + Q[v]);
+    for (int v = 0; v < V; ++v) Q[v] = fmaf(ga[AV == 1 ? 0 : v], s1, s0) * (ry[k][v] + Q[v]);
   }
   if (!WIDE) {
     wave_join<V, AV, false>(p, A, B, closed, eA, eB, eclosed);
@@ -174,10 +169,10 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
   mcut = again<WIDE>(mcut);
   first = again<WIDE>(first);
   last = again<WIDE>(last);
-  // a and b are computed again, not kept beside g and x
-  asm volatile("" : "+v"(s1), "+v"(s0));
-  alpha = __builtin_amdgcn_readfirstlane(again<false>(alpha));
+#pragma unroll
+  for (int k = 0; k < K; ++k) x[k].again(), g[k].again(), ry[k].again();
   // from the last row to the first: l takes the place of gy, x and the gates stay
+  float lam[K][V];
   const Turn<XT, V> tx(p.D, RL);
   const Turn<GT, AV> tg(p.G, RL);
 #pragma unroll
@@ -185,12 +180,14 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
     const ll at = r.p0 + k * r.step;
     float o[V];
     cut_at<V, WIDE>(p, k, mcut, last, gfinal, at, l.c, m);
+    float ga[AV];
+    gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float gav = ga[k][AV == 1 ? 0 : v];
-      g[k][v] += m[v];
-      o[v] = alpha ? gav * g[k][v] : g[k][v];
-      m[v] = fmaf(gav, s1, s0) * g[k][v];
+      const float gav = ga[AV == 1 ? 0 : v], z = ry[k][v] + m[v];
+      lam[k][v] = z;
+      o[v] = alpha ? gav * z : z;
+      m[v] = fmaf(gav, s1, s0) * z;
     }
     if (dx && l.ok) {
       if (turned) tx.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(o));
@@ -202,16 +199,19 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
   if (!dgate) return;
   // from the first row to the last: the states in front of the rows, and the gate's gradient
   float sums[K];
-  Vec<GT, AV> og[K];
+  Raw<GT, AV> og[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) x[k].again(), g[k].again();
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const ll at = r.p0 + k * r.step;
-    float d[V];
+    float d[V], ga[AV];
+    gates_of<GT, AV>(g[k], p.form, ga);
     cut_at<V, WIDE>(p, k, cut, first, p.h0, at, l.c, h);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float gav = ga[k][AV == 1 ? 0 : v];
-      d[v] = g[k][v] * (alpha ? x[k][v] - h[v] : logs ? gav * h[v] : h[v]);
+      const float gav = ga[AV == 1 ? 0 : v];
+      d[v] = lam[k][v] * (alpha ? x[k][v] - h[v] : logs ? gav * h[v] : h[v]);
       h[v] = fmaf(fmaf(gav, s1, s0), h[v], alpha ? gav * x[k][v] : x[k][v]);
     }
     if (!SHARED) {
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
   }
   if (SHARED) {
     if (p.LP >= K && (p.LP & (p.LP - 1)) == 0 && !turned) {
-      const float s = head_sums_pow2(sums, l.wl, p.LP);
-      const int k = (l.wl & 1) * 4 + (l.wl & 2) + (l.wl >> 2 & 1);
+      const float s = head_sums_pow2<K>(sums, l.wl, p.LP);
+      const int k = __brev(l.wl) >> (33 - __ffs(K));
       const ll at = r.p0 + k * r.step;
       if (l.wl < K && l.head && ((r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1)))) {
         if (dgate_parts) dgate_parts[((ll)l.part * p.n_rows + at) * p.G + l.g] = s;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
       }
       return;
     }
-    head_sums(sums, l.wl, p.LP);
+    head_sums<K>(sums, l.wl, p.LP);
     if (!turned) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(512, BWD_WAVES) scan_bwd_kernel(ScanArgs p, co
       return;
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k) og[k].v[0] = from_f<GT>(sums[k]);
+    for (int k = 0; k < K; ++k) og[k] = round_v<GT, AV>(&sums[k]);
   }
   if (turned) {
     wave_fence();

@@ -6,8 +6,9 @@ using namespace tfscan;
 
 namespace {
 
+
 template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
-__global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __restrict__ y, float* __restrict__ final, float* __restrict__ carry) {
+__global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARED ? 4 : 3 : 3) scan_fwd_kernel(ScanArgs p, XT* __restrict__ y, float* __restrict__ final, float* __restrict__ carry) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
   __shared__ unsigned s_ticket;
   __shared__ int s_closed[8], s_opened;
@@ -29,8 +30,8 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
   const ll w0 = t0 + (ll)(p.reverse ? nw - 1 - wave : wave) * RL * K;
   const int block = p.reverse ? RL - 1 - rl : rl;
   const bool full = t0 >= lo && t0 + T <= hi, turned = !WIDE && p.narrow && full;
-  Vec<XT, V> rx[K];
-  Vec<GT, AV> rg[K];
+  Raw<XT, V> x[K];
+  Raw<GT, AV> g[K];
   unsigned first, last;
   if (turned) {
     Turn<XT, V> tx(p.D, RL);
@@ -38,30 +39,37 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
     tx.load(static_cast<const XT*>(p.x) + w0 * p.D);
     tg.load(static_cast<const GT*>(p.gate) + w0 * p.G);
     r.bits(p, hi, first, last);
-    tx.to_rows(buf, p.D, block, l.c, p.reverse, rx);
-    tg.to_rows(buf, p.G, block, l.g, p.reverse, rg);
+    tx.to_rows(buf, p.D, block, l.c, p.reverse, x);
+    tg.to_rows(buf, p.G, block, l.g, p.reverse, g);
   } else {
-    direct_rows<XT, V, WIDE>(p, static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, rx);
-    direct_rows<GT, AV, WIDE>(p, static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, rg);
+    direct_rows<XT, V, WIDE>(static_cast<const XT*>(p.x), p.ld_x, r, l.c, full, x);
+    direct_rows<GT, AV, WIDE>(static_cast<const GT*>(p.gate), p.ld_gate, r, l.g, full, g);
     r.bits(p, hi, first, last);
   }
-  float a[K][AV], b[K][V];
+  // a row's a and b: in place of g and x where those are fp32 (40001 x 512 in two sequences: 62 us, 73 with both computed in either pass), from
+  // the packed values each time where they are not
+  constexpr bool WHOLE = sizeof(XT) == 4;
+  const bool alpha = p.form == TF_GATE_ALPHA;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
+    gates_kept<GT, AV>(g[k], p.form);
+    if (WHOLE && alpha) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) b[k][v] = to_f(rx[k].v[v]);
+      for (int v = 0; v < V; ++v) x[k].w[v] = __builtin_bit_cast(unsigned, x[k][v] * g[k][AV == 1 ? 0 : v]);
 #pragma unroll
-    for (int v = 0; v < AV; ++v) a[k][v] = to_f(rg[k].v[v]);
-    if (p.form == TF_GATE_LOG) {
-#pragma unroll
-      for (int v = 0; v < AV; ++v) a[k][v] = exp_gate(a[k][v]);
-    } else if (p.form == TF_GATE_ALPHA) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) b[k][v] *= a[k][AV == 1 ? 0 : v];
-#pragma unroll
-      for (int v = 0; v < AV; ++v) a[k][v] = 1.f - a[k][v];
+      for (int v = 0; v < AV; ++v) g[k].w[v] = __builtin_bit_cast(unsigned, 1.f - g[k][v]);
     }
   }
+  const float s1 = alpha ? -1.f : 1.f, s0 = alpha ? 1.f : 0.f;
+  auto terms = [&](int k, float (&a)[AV], float (&b)[V]) {
+    gates_of<GT, AV>(g[k], p.form, a);
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[v] = !WHOLE && alpha ? a[AV == 1 ? 0 : v] * x[k][v] : x[k][v];
+    if (!WHOLE) {
+#pragma unroll
+      for (int v = 0; v < AV; ++v) a[v] = fmaf(a[v], s1, s0);
+    }
+  };
   // a first row begins from h0 (or 0), a row of no segment from 0: it holds b = 0 and leaves 0
   unsigned cut = first | (~r.valid & ((1u << K) - 1));
   float A[AV], B[V], eA[AV], eB[V];
@@ -73,10 +81,12 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     cut_at<V, WIDE>(p, k, cut, first, p.h0, r.p0 + k * r.step, l.c, B);
+    float a[AV], b[V];
+    terms(k, a, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) B[v] = fmaf(a[k][AV == 1 ? 0 : v], B[v], b[k][v]);
+    for (int v = 0; v < V; ++v) B[v] = fmaf(a[AV == 1 ? 0 : v], B[v], b[v]);
 #pragma unroll
-    for (int v = 0; v < AV; ++v) A[v] *= a[k][v];
+    for (int v = 0; v < AV; ++v) A[v] *= a[v];
   }
   if (!WIDE) wave_join<V, AV, false>(p, A, B, closed, eA, eB, eclosed);
   if (rl == RL - 1) {
@@ -100,12 +110,18 @@ __global__ void __launch_bounds__(512, 4) scan_fwd_kernel(ScanArgs p, XT* __rest
   const Turn<XT, V> ty(p.D, RL);
   cut = again<WIDE>(cut);
   first = again<WIDE>(first);
+  if (!WHOLE) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) x[k].again(), g[k].again();
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const ll at = r.p0 + k * r.step;
     cut_at<V, WIDE>(p, k, cut, first, p.h0, at, l.c, h);
+    float a[AV], b[V];
+    terms(k, a, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][AV == 1 ? 0 : v], h[v], b[k][v]);
+    for (int v = 0; v < V; ++v) h[v] = fmaf(a[AV == 1 ? 0 : v], h[v], b[v]);
     if (l.ok) {
       if (turned) ty.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(h));
       else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h);

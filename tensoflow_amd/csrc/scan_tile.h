@@ -82,54 +82,105 @@ typedef __bf16 bf16;
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
 
+// V neighbours of a row as they come from memory, in whole words: 16-bit values stay packed and are widened where they are used
 template <typename T, int V>
-struct alignas((V & (V - 1)) ? sizeof(T) : sizeof(T) * V) Vec {
-  T v[V];
-};
-// Stored as whole words: the compiler takes a vector of 16-bit values apart into stores of single ones (65536 x 1024 bf16: 1.17 million store
-// instructions in place of 0.29), unless their words are beyond its sight.
-template <typename T, int V>
-__device__ __forceinline__ void put_words(void* p, const Vec<T, V>& r) {
-  constexpr int BYTES = sizeof(T) * V;
-  if constexpr (BYTES % 4 == 0) {
-    typedef unsigned u2 __attribute__((ext_vector_type(2)));
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    constexpr int N = BYTES / 4;
-    unsigned w[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (sizeof(T) == 4) {
-        w[i] = __builtin_bit_cast(unsigned, r.v[i]);
-      } else {
-        w[i] = __builtin_bit_cast(unsigned short, r.v[2 * i]) | (unsigned)__builtin_bit_cast(unsigned short, r.v[2 * i + 1]) << 16;
-        asm("" : "+v"(w[i]));
-      }
-    }
-    if constexpr (N == 4) *static_cast<u4*>(p) = u4{w[0], w[1], w[2], w[3]};
-    else if constexpr (N == 2) *static_cast<u2*>(p) = u2{w[0], w[1]};
-    else
-#pragma unroll
-      for (int i = 0; i < N; ++i) static_cast<unsigned*>(p)[i] = w[i];
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) static_cast<T*>(p)[v] = r.v[v];
+struct Raw {
+  static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
+  unsigned w[N];
+  __device__ __forceinline__ float operator[](int v) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[v]);
+    else return (float)__builtin_bit_cast(T, (unsigned short)(v & 1 ? w[v / 2] >> 16 : w[v / 2]));
   }
-}
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_v(const T* p) { return *reinterpret_cast<const Vec<T, V>*>(p); }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> round_v(const float* f) {
-  Vec<T, V> r;
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int v = 0; v < V; ++v) r.v[v] = from_f<T>(f[v]);
+    for (int i = 0; i < N; ++i) w[i] = 0;
+  }
+  // as if read anew: what was computed from it before is computed again, not kept beside it
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_v(const T* p) {
+  Raw<T, V> r;
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES == 16) {
+    const u4 q = *reinterpret_cast<const u4*>(p);
+    r.w[0] = q.x, r.w[1] = q.y, r.w[2] = q.z, r.w[3] = q.w;
+  } else if constexpr (BYTES == 8) {
+    const u2 q = *reinterpret_cast<const u2*>(p);
+    r.w[0] = q.x, r.w[1] = q.y;
+  } else if constexpr (sizeof(T) == 4 || BYTES == 4) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::N; ++i) r.w[i] = reinterpret_cast<const unsigned*>(p)[i];
+  } else {
+    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+    r.w[0] = s[0];
+    if constexpr (V == 3) r.w[0] |= (unsigned)s[1] << 16, r.w[1] = s[2];
+  }
   return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float* f) { put_words<T, V>(p, round_v<T, V>(f)); }
+__device__ __forceinline__ Raw<T, V> round_v(const float* f) {
+  Raw<T, V> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.w[v] = __builtin_bit_cast(unsigned, f[v]);
+  } else {
+    r.zero();
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.w[v / 2] |= (unsigned)__builtin_bit_cast(unsigned short, from_f<T>(f[v])) << (v & 1 ? 16 : 0);
+    // beyond the compiler's sight: it would take the words apart into stores of single values
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::N; ++i) asm("" : "+v"(r.w[i]));
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void put_v(T* p, const Raw<T, V>& r) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES == 16) *reinterpret_cast<u4*>(p) = u4{r.w[0], r.w[1], r.w[2], r.w[3]};
+  else if constexpr (BYTES == 8) *reinterpret_cast<u2*>(p) = u2{r.w[0], r.w[1]};
+  else if constexpr (sizeof(T) == 4 || BYTES == 4) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::N; ++i) reinterpret_cast<unsigned*>(p)[i] = r.w[i];
+  } else {
+    unsigned short* s = reinterpret_cast<unsigned short*>(p);
+    s[0] = (unsigned short)r.w[0];
+    if constexpr (V == 3) s[1] = (unsigned short)(r.w[0] >> 16), s[2] = (unsigned short)r.w[1];
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float* f) { put_v<T, V>(p, round_v<T, V>(f)); }
 
 __device__ __forceinline__ unsigned clean(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
 // exp(g) = 2^(g log2 e) on the hardware's 2^x (1 ulp): g's product is rounded once, a relative error of the result of |g| 2^-24
 __device__ __forceinline__ float exp_gate(float g) { return __builtin_amdgcn_exp2f(g * 1.44269504088896341f); }
+
+// a row's gates as ga (g of TF_GATE_ALPHA, else a): a = ga * s1 + s0, exact where nothing is to be done; fp32 ones are kept in that form
+template <typename GT, int AV>
+__device__ __forceinline__ void gates_kept(Raw<GT, AV>& r, int form) {
+  if constexpr (sizeof(GT) == 4) {
+    if (form == TF_GATE_LOG) {
+#pragma unroll
+      for (int v = 0; v < AV; ++v) r.w[v] = __builtin_bit_cast(unsigned, exp_gate(r[v]));
+    }
+  }
+}
+template <typename GT, int AV>
+__device__ __forceinline__ void gates_of(const Raw<GT, AV>& r, int form, float (&ga)[AV]) {
+#pragma unroll
+  for (int v = 0; v < AV; ++v) ga[v] = r[v];
+  if constexpr (sizeof(GT) == 2) {
+    if (form == TF_GATE_LOG) {
+#pragma unroll
+      for (int v = 0; v < AV; ++v) ga[v] = exp_gate(ga[v]);
+    }
+  }
+}
 
 // words and ends are written and read past the caches of one XCD, each word whole: no fence orders anything else
 __device__ __forceinline__ ull peek(const ull* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -143,30 +194,35 @@ struct Map {
   float A = 1.f, B = 0.f;
   bool closed = false;
 };
-// the n < GRP words of channel c before row `at` of D, the nearest first: all asked for at once, those that are not there yet again
-__device__ __forceinline__ void join_words(const ull* at, int D, int c, int n, Map& m) {
+// the n < GRP words of channel c before row `at` of D, the nearest first
+struct Words {
   ull w[GRP - 1];
+  __device__ __forceinline__ void ask(const ull* at, int D, int c, int n) {
 #pragma unroll
-  for (int i = 0; i < GRP - 1; ++i) w[i] = i < n ? peek(at - (ll)(i + 1) * D + c) : 0;
-  while (true) {
-    bool missing = false;
-#pragma unroll
-    for (int i = 0; i < GRP - 1; ++i) missing |= w[i] == EMPTY;
-    if (!__any(missing)) break;
-    __builtin_amdgcn_s_sleep(1);
-#pragma unroll
-    for (int i = 0; i < GRP - 1; ++i)
-      if (w[i] == EMPTY) w[i] = peek(at - (ll)(i + 1) * D + c);
+    for (int i = 0; i < GRP - 1; ++i) w[i] = i < n ? peek(at - (ll)(i + 1) * D + c) : 0;
   }
+  // those that are not there yet again, until they are; then joined
+  __device__ __forceinline__ void join(const ull* at, int D, int c, int n, Map& m) {
+    while (true) {
+      bool missing = false;
 #pragma unroll
-  for (int i = 0; i < GRP - 1; ++i) {
-    if (i >= n || m.closed) break;
-    const unsigned a = (unsigned)(w[i] >> 32);
-    m.B = fmaf(m.A, __uint_as_float((unsigned)w[i]), m.B);
-    m.closed = __builtin_amdgcn_readfirstlane(a) == CLOSED;
-    m.A *= __uint_as_float(a);
+      for (int i = 0; i < GRP - 1; ++i) missing |= w[i] == EMPTY;
+      if (!__any(missing)) break;
+      __builtin_amdgcn_s_sleep(1);
+#pragma unroll
+      for (int i = 0; i < GRP - 1; ++i)
+        if (w[i] == EMPTY) w[i] = peek(at - (ll)(i + 1) * D + c);
+    }
+#pragma unroll
+    for (int i = 0; i < GRP - 1; ++i) {
+      if (i >= n || m.closed) break;
+      const unsigned a = (unsigned)(w[i] >> 32);
+      m.B = fmaf(m.A, __uint_as_float((unsigned)w[i]), m.B);
+      m.closed = __builtin_amdgcn_readfirstlane(a) == CLOSED;
+      m.A *= __uint_as_float(a);
+    }
   }
-}
+};
 // posts tile q's own map of channel c -> the state in front of it
 __device__ __forceinline__ float chain(const ScanArgs& p, int q, int c, float A, float B, bool closed, bool opened) {
   const int D = p.D, iq = q % GRP, g = q / GRP, ig = g % GRP, s = g / GRP;
@@ -175,13 +231,26 @@ __device__ __forceinline__ float chain(const ScanArgs& p, int q, int c, float A,
   post(words + c, word_of(A, B, closed));
   Map m;
   m.closed = opened;
-  if (!opened && iq) join_words(words, D, c, iq, m);
+  Words w;
+  if (!opened && iq) {
+    w.ask(words, D, c, iq);
+    w.join(words, D, c, iq, m);
+  }
   if (iq == GRP - 1) post(groups + c, closed ? word_of(A, B, true) : word_of(A * m.A, fmaf(A, m.B, B), m.closed));
-  if (!m.closed && ig) join_words(groups, D, c, ig, m);
+  unsigned e = 0;
+  if (!m.closed) {
+    if (s) e = peek(ends - D + c);
+    if (ig) {
+      w.ask(groups, D, c, ig);
+      w.join(groups, D, c, ig, m);
+    }
+  }
   float h = m.B;
   if (!m.closed && s) {
-    unsigned e;
-    while (__any((e = peek(ends - D + c)) == 0xffffffffu)) __builtin_amdgcn_s_sleep(1);
+    while (__any(e == 0xffffffffu)) {
+      __builtin_amdgcn_s_sleep(1);
+      e = peek(ends - D + c);
+    }
     h = fmaf(m.A, __uint_as_float(e), m.B);
   }
   if (iq == GRP - 1 && ig == GRP - 1) post(ends + c, clean(closed ? B : fmaf(A, h, B)));
@@ -320,7 +389,6 @@ __device__ __forceinline__ void wave_fence() {
 template <typename T, int V>
 struct Turn {
   static constexpr int NC = (K * V * (int)sizeof(T) + 15) / 16;  // 16-byte pieces of a lane, at most
-  typedef unsigned u4 __attribute__((ext_vector_type(4)));
   u4 piece[NC];
   int unit, magic, count;  // pieces of a lane's K rows; of the wave
   __device__ __forceinline__ Turn(int width, int RL) {
@@ -335,7 +403,7 @@ struct Turn {
     for (int j = 0; j < NC; ++j) piece[j] = j * 64 + lane < count ? reinterpret_cast<const u4*>(rows)[j * 64 + lane] : u4{0, 0, 0, 0};
   }
   // pieces -> the lane's rows; block: which K rows of the wave's, in memory's order
-  __device__ __forceinline__ void to_rows(char* buf, int width, int block, int c, bool reverse, Vec<T, V> (&out)[K]) {
+  __device__ __forceinline__ void to_rows(char* buf, int width, int block, int c, bool reverse, Raw<T, V> (&out)[K]) {
     const int lane = threadIdx.x & 63;
     wave_fence();
 #pragma unroll
@@ -344,11 +412,11 @@ struct Turn {
     wave_fence();
     const T* at = reinterpret_cast<const T*>(buf + block * (unit + 1) * 16) + c;
 #pragma unroll
-    for (int k = 0; k < K; ++k) out[k] = *reinterpret_cast<const Vec<T, V>*>(at + (reverse ? K - 1 - k : k) * width);
+    for (int k = 0; k < K; ++k) out[k] = load_v<T, V>(at + (reverse ? K - 1 - k : k) * width);
   }
   // and back: the lane's row k
-  __device__ __forceinline__ void put(char* buf, int width, int block, int c, bool reverse, int k, const Vec<T, V>& v) const {
-    put_words<T, V>(reinterpret_cast<T*>(buf + block * (unit + 1) * 16) + (reverse ? K - 1 - k : k) * width + c, v);
+  __device__ __forceinline__ void put(char* buf, int width, int block, int c, bool reverse, int k, const Raw<T, V>& v) const {
+    put_v<T, V>(reinterpret_cast<T*>(buf + block * (unit + 1) * 16) + (reverse ? K - 1 - k : k) * width + c, v);
   }
   __device__ __forceinline__ void store(const char* buf, T* rows) const {
     const int lane = threadIdx.x & 63;
@@ -361,7 +429,7 @@ struct Turn {
 
 // the lane's rows as they lie in memory
 template <typename T, int V, bool WIDE>
-__device__ __forceinline__ void direct_rows(const ScanArgs& p, const T* base, ll ld, const Rows<WIDE>& r, int c, bool full, Vec<T, V> (&out)[K]) {
+__device__ __forceinline__ void direct_rows(const T* base, ll ld, const Rows<WIDE>& r, int c, bool full, Raw<T, V> (&out)[K]) {
   if (full) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -372,12 +440,8 @@ __device__ __forceinline__ void direct_rows(const ScanArgs& p, const T* base, ll
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const T* row = base + (r.p0 + k * r.step) * ld;
-      if (r.valid >> k & 1) {
-        out[k] = load_v<T, V>(row + c);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[k].v[v] = from_f<T>(0.f);
-      }
+      out[k].zero();
+      if (r.valid >> k & 1) out[k] = load_v<T, V>(row + c);
     }
   }
 }
@@ -451,6 +515,7 @@ __device__ __forceinline__ void join_waves(const ScanArgs& p, int q, int slab, i
     if (p.ticket) {
       float A = 1.f, B = 0.f;
       bool closed = false;
+#pragma unroll 4
       for (int i = 0; i < nw; ++i) {
         const int w = DOWN ? nw - 1 - i : i;
         const float a = sA[w * p.W + t], b = sB[w * p.W + t];

@@ -12,8 +12,8 @@ typedef unsigned long long ull;
 // Up to SMALL segments every workgroup sums the lengths by itself and finds its rows' segments in LDS: ONE launch, where the sums' own would cost
 // as much again (1024 segments, 130003 rows: 9.6 -> 6.4 us of kernels).  More segments: sums, offsets, rows.
 constexpr int SMALL = 2048;
-constexpr int CHUNK = 4096;  // lengths of a workgroup of the sums
-constexpr int WAVE_ROWS = 512;
+constexpr int CHUNK = 2048;  // lengths of a workgroup of the sums
+constexpr int WAVE_ROWS = 1024;  // rows of a wave of the rows
 
 __device__ __forceinline__ ll seg_len(const ll* __restrict__ lengths, ll s, ll n_rows) { return min(max(lengths[s], 0ll), n_rows); }
 
@@ -153,24 +153,31 @@ __global__ void __launch_bounds__(256) seg_offsets_kernel(const ll* __restrict__
   base = total;
   block_exclusive<4>(bbase, part, total);
   bbase = total;
-  for (int k = 0; k < CHUNK / 256; ++k) {
-    const ll s = (ll)blockIdx.x * CHUNK + k * 256 + threadIdx.x;
-    const ll v = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
-    const ll at = min(base + block_exclusive<4>(v, part, total), n_rows);
-    base += total;
-    ll bat = 0;
-    if (b.rows) {
-      bat = bbase + block_exclusive<4>(blocks_of(b, v), part, total);
-      bbase += total;
+  constexpr int PER = CHUNK / 256;
+  ll v[PER], sum = 0, bsum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const ll s = (ll)blockIdx.x * CHUNK + threadIdx.x * PER + k;
+    v[k] = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
+    sum += v[k];
+    if (b.rows) bsum += blocks_of(b, v[k]);
+  }
+  base += block_exclusive<4>(sum, part, total);
+  if (b.rows) bbase += block_exclusive<4>(bsum, part, total);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const ll s = (ll)blockIdx.x * CHUNK + threadIdx.x * PER + k, at = min(base, n_rows);
+    if (s < n_seg) {
+      offsets[s] = at;
+      if (b.rows) block_first[s] = bbase;
+      if (s == n_seg - 1) offsets[n_seg] = min(at + v[k], n_rows);
+      if (starts && v[k] > 0 && at < n_rows) {
+        atomicOr(starts + (at >> 6), 1ull << (at & 63));
+        if (index) index[at] = s;
+      }
     }
-    if (s >= n_seg) continue;
-    offsets[s] = at;
-    if (b.rows) block_first[s] = bat;
-    if (s == n_seg - 1) offsets[n_seg] = min(at + v, n_rows);
-    if (starts && v > 0 && at < n_rows) {
-      atomicOr(starts + (at >> 6), 1ull << (at & 63));
-      if (index) index[at] = s;
-    }
+    base += v[k];
+    if (b.rows) bbase += blocks_of(b, v[k]);
   }
 }
 
@@ -188,41 +195,61 @@ __device__ __forceinline__ ll wave_seg_of(const ll* __restrict__ offsets, ll n_s
   return lo;
 }
 
-// every row from the start bits: a row belongs to the last start at or before it, within its 64 rows or carried from before
+// Every row from the start bits: a row belongs to the last start at or before it, among the wave's 128 rows or carried from before.  A lane has two rows
+// side by side, stored as one piece of 16 bytes (33.3 million rows, 640000 segments, two tables: 153 us with a row and 8 bytes a lane).
+typedef ll ll2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void put2(ll* p, ll i, ll n, bool pair, ll a, ll b) {
+  if (pair && i + 1 < n) {
+    __builtin_nontemporal_store(ll2{a, b}, reinterpret_cast<ll2*>(p + i));
+  } else {
+    if (i < n) p[i] = a;
+    if (i + 1 < n) p[i + 1] = b;
+  }
+}
 __global__ void __launch_bounds__(256) seg_rows_kernel(const ll* __restrict__ offsets, const ll* __restrict__ block_first, ll n_seg, ll n_rows,
-                                                       const ull* __restrict__ starts, ll* index, ll* __restrict__ position, Blocks b) {
-  constexpr int N = WAVE_ROWS / 64;
+                                                       const ull* __restrict__ starts, ll* index, ll* __restrict__ position, Blocks b, bool pair) {
+  constexpr int N = WAVE_ROWS / 128;
   const int lane = threadIdx.x & 63;
-  const ll row0 = ((ll)blockIdx.x * 4 + (threadIdx.x >> 6)) * WAVE_ROWS, end = offsets[n_seg];
+  const ll row0 = ((ll)blockIdx.x * 4 + (threadIdx.x >> 6)) * WAVE_ROWS, end = offsets[n_seg], words = (n_rows + 63) >> 6;
   if (row0 >= n_rows) return;
-  ull word[N];
-  ll seg[N];
+  // the two start bits of the lane's rows in each of the wave's stretches of 128, and the segments that begin there
+  unsigned two[N];
+  ll s0[N], s1[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) word[k] = row0 + 64 * k < n_rows ? starts[(row0 >> 6) + k] : 0;
+  for (int k = 0; k < N; ++k) {
+    const ll w = (row0 >> 6) + 2 * k + (lane >> 5);
+    two[k] = w < words ? (unsigned)(starts[w] >> (2 * lane & 63)) & 3 : 0;
+  }
 #pragma unroll
-  for (int k = 0; k < N; ++k) seg[k] = index && (word[k] >> lane & 1) ? index[row0 + 64 * k + lane] : 0;
+  for (int k = 0; k < N; ++k) {
+    const ll i = row0 + 128 * k + 2 * lane;
+    s0[k] = index && (two[k] & 1) ? index[i] : 0;
+    s1[k] = index && (two[k] & 2) ? index[i + 1] : 0;
+  }
   ll cseg = -1, cstart = 0;
-  if (!(word[0] & 1) && row0 < end) {
+  if (!(__builtin_amdgcn_readfirstlane(two[0]) & 1) && row0 < end) {
     cseg = wave_seg_of(offsets, n_seg, row0);
     cstart = offsets[cseg];
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const ll i = row0 + 64 * k + lane;
-    const ull upto = word[k] & (~0ull >> (63 - lane));
-    const int src = upto ? 63 - __clzll((long long)upto) : 0, lastsrc = word[k] ? 63 - __clzll((long long)word[k]) : 0;
-    const ll near = __shfl(seg[k], src), lastseg = __shfl(seg[k], lastsrc);
-    const ll s = upto ? near : cseg, p = i - (upto ? row0 + 64 * k + src : cstart);
-    if (word[k]) {
-      cseg = lastseg;
-      cstart = row0 + 64 * k + lastsrc;
+    const ll base = row0 + 128 * k, i = base + 2 * lane;
+    const ull any = __ballot(two[k] != 0), odd = __ballot(two[k] & 2), before = any & ((1ull << lane) - 1);
+    const ll mine = two[k] & 2 ? s1[k] : s0[k];
+    // the last start in front of the lane's rows, and the last of all
+    const int src = before ? 63 - __clzll((long long)before) : 0, top = any ? 63 - __clzll((long long)any) : 0;
+    const ll got = __shfl(mine, src), last = __shfl(mine, top);
+    const ll ps = before ? got : cseg, pstart = before ? base + 2 * src + (ll)(odd >> src & 1) : cstart;
+    const ll sa = two[k] & 1 ? s0[k] : ps, pa = two[k] & 1 ? 0 : i - pstart;
+    const ll sb = two[k] & 2 ? s1[k] : sa, pb = two[k] & 2 ? 0 : pa + 1;
+    if (any) {
+      cseg = last;
+      cstart = base + 2 * top + (ll)(odd >> top & 1);
     }
-    if (i < n_rows) {
-      const bool ok = i < end;
-      if (index) index[i] = ok ? s : -1;
-      if (position) position[i] = ok ? p : -1;
-      if (b.slots) b.slots[i] = ok ? slot_of(b, block_first[s], p) : -1;
-    }
+    const bool oka = i < end, okb = i + 1 < end;
+    if (index) put2(index, i, n_rows, pair, oka ? sa : -1, okb ? sb : -1);
+    if (position) put2(position, i, n_rows, pair, oka ? pa : -1, okb ? pb : -1);
+    if (b.slots) put2(b.slots, i, n_rows, pair, oka ? slot_of(b, block_first[sa], pa) : -1, okb ? slot_of(b, block_first[sb], pb) : -1);
   }
 }
 
@@ -297,12 +324,13 @@ extern "C" int tf_segment_tables(const int64_t* lengths, int64_t n_segments, int
     ll* sums = (ll*)workspace;
     ll* first = sums + 2 * chunks_of(n_segments);
     const unsigned grid = (unsigned)chunks_of(n_segments);
+    const bool pair = (((size_t)index | (size_t)position | (size_t)slots) & 15) == 0;
     seg_sums_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ull*)starts, starts ? (n_rows + 63) >> 6 : 0);
     seg_offsets_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ll*)offsets, first, (ll*)index, (ull*)starts);
     if (cells) seg_blocks_kernel<<<(unsigned)((cells + 255) / 256), 256, 0, st>>>((const ll*)lengths, first, n_segments, n_rows, b);
     if (n_rows > 0 && (index || position))
       seg_rows_kernel<<<(unsigned)((n_rows + 4 * WAVE_ROWS - 1) / (4 * WAVE_ROWS)), 256, 0, st>>>((const ll*)offsets, first, n_segments, n_rows, (const ull*)starts,
-                                                                                              (ll*)index, (ll*)position, b);
+                                                                                              (ll*)index, (ll*)position, b, pair);
   }
   TF_LAUNCH_CHECK("tf_segment_tables");
   return TF_OK;
