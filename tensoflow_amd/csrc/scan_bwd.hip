@@ -95,6 +95,29 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
   const float s1 = alpha ? -1.f : 1.f, s0 = alpha ? 1.f : 0.f;
   const unsigned none = ~r.valid & ((1u << K) - 1);
   unsigned cut = first | none, mcut = last | none;
+  // for all of a lane's rows at once: what comes from behind a segment's end, added to gy where that is fp32; the states that segments begin from
+  const float *h0 = p.h0, *gf = gfinal;
+  constexpr bool WHOLE = sizeof(XT) == 4;
+  int seg0[K];
+  float begin[K][V];
+  if (!WIDE && WHOLE && gf) {
+    if (__any(last)) {
+      int seg[K];
+      float s[K][V];
+      segs_of<WIDE>(p, r, last, seg);
+      states_of<V>(p, gf, seg, l.c, s);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) ry[k].w[v] = __builtin_bit_cast(unsigned, seg[k] >= 0 ? ry[k][v] + s[k][v] : ry[k][v]);
+    }
+    gf = nullptr;
+  }
+  const bool some = !WIDE && (p.h0 || dh0) && __any(first);
+  if (some) segs_of<WIDE>(p, r, first, seg0);
+  const bool began = !WIDE && WHOLE && h0 && some;
+  if (began) states_of<V>(p, h0, seg0, l.c, begin);
+  if (!WIDE && WHOLE) h0 = nullptr;
   float A[AV], B[V], eA[AV], eB[V], P[AV], Q[V], eP[AV], eQ[V];
   bool closed = cut != 0, eclosed, mclosed = mcut != 0, emclosed;
 #pragma unroll
@@ -103,7 +126,11 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
   for (int v = 0; v < V; ++v) B[v] = Q[v] = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    cut_at<V, WIDE>(p, k, cut, first, p.h0, r.p0 + k * r.step, l.c, B);
+    cut_at<V, WIDE>(p, k, cut, first, h0, r.p0 + k * r.step, l.c, B);
+    if (!WIDE && WHOLE && began) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) B[v] = seg0[k] >= 0 ? begin[k][v] : B[v];
+    }
     float ga[AV];
     gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
@@ -118,7 +145,7 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
   for (int v = 0; v < AV; ++v) P[v] = A[v];
 #pragma unroll
   for (int k = K - 1; k >= 0; --k) {
-    cut_at<V, WIDE>(p, k, mcut, last, gfinal, r.p0 + k * r.step, l.c, Q);
+    cut_at<V, WIDE>(p, k, mcut, last, gf, r.p0 + k * r.step, l.c, Q);
     float ga[AV];
     gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
@@ -179,7 +206,7 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
   for (int k = K - 1; k >= 0; --k) {
     const ll at = r.p0 + k * r.step;
     float o[V];
-    cut_at<V, WIDE>(p, k, mcut, last, gfinal, at, l.c, m);
+    cut_at<V, WIDE>(p, k, mcut, last, gf, at, l.c, m);
     float ga[AV];
     gates_of<GT, AV>(g[k], p.form, ga);
 #pragma unroll
@@ -193,10 +220,16 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
       if (turned) tx.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(o));
       else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((dx + at * p.D) + l.c, o);
     }
-    if (dh0 && l.ok && (first >> k & 1)) put_state<V>(p, dh0, at, l.c, m);
+    if (WIDE) {
+      if (dh0 && l.ok && (first >> k & 1)) put_state<V>(p, dh0, at, l.c, m);
+    } else if (dh0 && some && l.ok && seg0[k] >= 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) dh0[(ll)seg0[k] * p.D + l.c + v] = m[v];
+    }
   }
   if (turned && dx) tx.store(buf, dx + w0 * p.D);
   if (!dgate) return;
+  if (began) states_of<V>(p, p.h0, seg0, l.c, begin);
   // from the first row to the last: the states in front of the rows, and the gate's gradient
   float sums[K];
   Raw<GT, AV> og[K];
@@ -207,7 +240,11 @@ __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const floa
     const ll at = r.p0 + k * r.step;
     float d[V], ga[AV];
     gates_of<GT, AV>(g[k], p.form, ga);
-    cut_at<V, WIDE>(p, k, cut, first, p.h0, at, l.c, h);
+    cut_at<V, WIDE>(p, k, cut, first, h0, at, l.c, h);
+    if (!WIDE && WHOLE && began) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = seg0[k] >= 0 ? begin[k][v] : h[v];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float gav = ga[AV == 1 ? 0 : v];

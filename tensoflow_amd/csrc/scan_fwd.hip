@@ -70,6 +70,22 @@ __global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARE
       for (int v = 0; v < AV; ++v) a[v] = fmaf(a[v], s1, s0);
     }
   };
+  // the states that segments begin from, for all of a lane's rows at once: b + a h0 in the place of b
+  const float* h0 = p.h0;
+  if (!WIDE && WHOLE && h0) {
+    if (__any(first)) {
+      int seg[K];
+      float s[K][V];
+      segs_of<WIDE>(p, r, first, seg);
+      states_of<V>(p, h0, seg, l.c, s);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          x[k].w[v] = __builtin_bit_cast(unsigned, seg[k] >= 0 ? fmaf(g[k][AV == 1 ? 0 : v], s[k][v], x[k][v]) : x[k][v]);
+    }
+    h0 = nullptr;
+  }
   // a first row begins from h0 (or 0), a row of no segment from 0: it holds b = 0 and leaves 0
   unsigned cut = first | (~r.valid & ((1u << K) - 1));
   float A[AV], B[V], eA[AV], eB[V];
@@ -80,7 +96,7 @@ __global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARE
   for (int v = 0; v < V; ++v) B[v] = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    cut_at<V, WIDE>(p, k, cut, first, p.h0, r.p0 + k * r.step, l.c, B);
+    cut_at<V, WIDE>(p, k, cut, first, h0, r.p0 + k * r.step, l.c, B);
     float a[AV], b[V];
     terms(k, a, b);
 #pragma unroll
@@ -108,6 +124,9 @@ __global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARE
     h[v] = WIDE ? s : eclosed ? eB[v] : fmaf(eA[AV == 1 ? 0 : v], s, eB[v]);
   }
   const Turn<XT, V> ty(p.D, RL);
+  int ends[K];
+  const bool some = !WIDE && final && __any(last);
+  if (some) segs_of<WIDE>(p, r, last, ends);
   cut = again<WIDE>(cut);
   first = again<WIDE>(first);
   if (!WHOLE) {
@@ -117,7 +136,7 @@ __global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARE
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const ll at = r.p0 + k * r.step;
-    cut_at<V, WIDE>(p, k, cut, first, p.h0, at, l.c, h);
+    cut_at<V, WIDE>(p, k, cut, first, h0, at, l.c, h);
     float a[AV], b[V];
     terms(k, a, b);
 #pragma unroll
@@ -125,7 +144,12 @@ __global__ void __launch_bounds__(512, SHARED || sizeof(XT) == 2 ? WIDE || SHARE
     if (l.ok) {
       if (turned) ty.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(h));
       else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h);
-      if (final && (last >> k & 1)) put_state<V>(p, final, at, l.c, h);
+      if (WIDE) {
+        if (final && (last >> k & 1)) put_state<V>(p, final, at, l.c, h);
+      } else if (some && ends[k] >= 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) final[(ll)ends[k] * p.D + l.c + v] = h[v];
+      }
     }
   }
   if (turned) ty.store(buf, y + w0 * p.D);

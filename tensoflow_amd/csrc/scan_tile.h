@@ -367,6 +367,24 @@ __device__ __forceinline__ void cut_at(const ScanArgs& p, int k, unsigned cut, u
   }
 }
 
+// The same for all rows of a lane at once, where lanes have rows of their own: row after row, each with a wait for its index and one for its state,
+// the edges of short segments cost more than the rest (8000003 x 4 fp32, 23 rows a segment: 160 us).  Lanes without an edge read a place that is there.
+template <bool WIDE>
+__device__ __forceinline__ void segs_of(const ScanArgs& p, const Rows<WIDE>& r, unsigned edge, int (&seg)[K]) {
+  ll v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = p.index[edge >> k & 1 ? r.p0 + k * r.step : 0];
+#pragma unroll
+  for (int k = 0; k < K; ++k) seg[k] = (edge >> k & 1) && v[k] >= 0 && v[k] < p.n_seg ? (int)v[k] : -1;
+}
+template <int V>
+__device__ __forceinline__ void states_of(const ScanArgs& p, const float* s, const int (&seg)[K], int c, float (&out)[K][V]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[k][v] = s[(ll)max(seg[k], 0) * p.D + c + v];
+}
+
 // segments without rows hand `from` (or 0) on to `to`: a wave looks at 64 of them and copies row after row
 __device__ __forceinline__ void empty_segments(const ScanArgs& p, ll wave, const float* from, float* to) {
   const int lane = threadIdx.x & 63;
