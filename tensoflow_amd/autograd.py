@@ -418,8 +418,7 @@ class GatedScanFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, x, h0, tables, form, reverse):
-        d = lambda t: None if t is None else t.detach()
-        y, final, carry = ops.gated_scan(d(gate), d(x), tables, d(h0), form, reverse, want_final=tables.index is not None, want_carry=True)
+        y, final, carry = ops.gated_scan(gate, x, tables, h0, form, reverse, want_final=tables.index is not None, want_carry=True)
         ctx.save_for_backward(gate, x, h0, carry)
         ctx.cfg = (tables, form, reverse)
         ctx.set_materialize_grads(False)

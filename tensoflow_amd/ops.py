@@ -526,16 +526,16 @@ class SegmentTables:
 
 
 def _on(*tensors):
-    """The stream to enqueue on: the current one of the tensors' device, which has to be the current device."""
+    """The raw stream to enqueue on: the current one of the tensors' device, which has to be the current device."""
     dev = tensors[0].device
     for t in tensors:
         if t is not None and t.device != dev:
             raise RuntimeError(f"tensors on {dev} and {t.device}: one device is wanted")
     if dev.type != "cuda":
         raise RuntimeError("a CUDA/HIP tensor is wanted (tensoflow_amd has no CPU path)")
-    if dev.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}: enter torch.cuda.device({dev.index})")
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    if dev.index != torch._C._cuda_getDevice():
+        raise RuntimeError(f"tensors on {dev}, but the current device is cuda:{torch._C._cuda_getDevice()}: enter torch.cuda.device({dev.index})")
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 _MOST_ROWS = 1 << 38
