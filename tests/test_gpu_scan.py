@@ -179,6 +179,54 @@ def test_scan_long(dev, d, g, t):
     run_case(dev, [1, 4100], d, g, t, "f32", "log", True, seed=d + 1, extra=1)
 
 
+@pytest.mark.parametrize("d,g,t,gt", [(387, 387, "f32", "f32"), (387, 3, "bf16", "f32"), (259, 1, "f16", "f16"), (514, 514, "bf16", "bf16"), (514, 257, "f32", "f32"),
+                                      (63, 63, "bf16", "f32"), (60, 60, "f16", "f16"), (62, 31, "bf16", "f32"), (774, 2, "bf16", "bf16")])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_odd_widths(dev, d, g, t, gt, reverse):
+    """Every width of a lane's vector, one workgroup and several across the channels, heads across workgroups, short rows of two types."""
+    for k, form in enumerate(("decay", "log", "alpha")):
+        run_case(dev, [70, 0, 3, 300, 1, 1, 140], d, g, t, gt, form, reverse, seed=d + k, extra=3 * k)
+
+
+@pytest.mark.parametrize("d,n,reverse", [(1, 3000001, False), (3, 1200007, True), (8, 400003, False), (64, 70001, True), (520, 9001, False)])
+def test_scan_many_tiles_exactly(dev, d, n, reverse):
+    """Decays of 1 and small whole numbers: every sum is exact in 24 bits in any order, so thousands of tiles have to give the running sums to the bit."""
+    from tensoflow_amd import ops
+    g = torch.Generator(device=dev).manual_seed(d)
+    cut = n // 3
+    ln = [cut, 0, 1, n - cut - 1]
+    x = torch.randint(-2, 3, (n, d), device=dev, generator=g).float()
+    gy = torch.randint(-2, 3, (n, d), device=dev, generator=g).float()
+    one = torch.ones(n, 1, device=dev)
+    tab = ops.segment_tables(torch.tensor(ln, device=dev), n)
+    sums = lambda v, back: torch.cat([(s.flip(0) if back else s).double().cumsum(0).flip([0] if back else []) for s in v.split([cut, 1, n - cut - 1])])
+    y, final, carry = ops.gated_scan(one, x, tab, None, "decay", reverse, want_final=True, want_carry=True)
+    want, lam = sums(x, reverse), sums(gy, not reverse)
+    assert float(want.abs().max()) < 2 ** 24 and float(lam.abs().max()) < 2 ** 24
+    assert torch.equal(y.double(), want)
+    ends = [0, cut, cut + 1] if reverse else [cut - 1, cut, n - 1]
+    assert torch.equal(final[[0, 2, 3]].double(), want[ends]) and bool((final[1] == 0).all())
+    gg, gx, gh = ops.gated_scan_bwd(one, x, tab, carry, gy, None, None, "decay", reverse)
+    assert torch.equal(gx.double(), lam)
+    ends = [cut - 1, cut, n - 1] if reverse else [0, cut, cut + 1]
+    assert torch.equal(gh[[0, 2, 3]].double(), lam[ends]) and bool((gh[1] == 0).all())
+    before = want - x.double()
+    part = lam * before
+    # each product is rounded once and at most d - 1 sums of theirs follow
+    assert bool(((gg.double() - part.sum(1, keepdim=True)).abs() <= d * 2.0 ** -24 * part.abs().sum(1, keepdim=True)).all())
+
+
+def test_scan_without_segments(dev):
+    from tensoflow_amd import ops
+    tab = ops.segment_tables(torch.zeros(0, dtype=torch.int64, device=dev), 300)
+    for d, gates in ((3, 1), (300, 300)):
+        x, gate = torch.full((300, d), float("nan"), device=dev), torch.full((300, gates), float("nan"), device=dev)
+        y, final, carry = ops.gated_scan(gate, x, tab, torch.zeros(0, d, device=dev), want_final=True, want_carry=True)
+        assert bool((y == 0).all()) and final.shape == (0, d)
+        gg, gx, gh = ops.gated_scan_bwd(gate, x, tab, carry, x, final, torch.zeros(0, d, device=dev))
+        assert bool((gg == 0).all()) and bool((gx == 0).all()) and gh.shape == (0, d)
+
+
 def test_scan_does_not_cross_segments(dev):
     """A neighbour's NaN, inf or overflow stays there: a first step selects its own state, it does not multiply the last one by 0."""
     from tensoflow_amd import ops
@@ -451,6 +499,20 @@ def test_step_after_step_is_the_scan(dev):
 
 
 # ---------------------------------------------------------------------------------------------- streams and graphs
+def test_step_strides(dev):
+    """Column slices of a fused projection, at even and odd places."""
+    from tensoflow_amd import ops
+    for b, d in ((3, 40), (80, 1024)):
+        for off in (0, 1, 4):
+            both = torch.randn(b, 2 * d + 9, device=dev).bfloat16()
+            x, g = both[:, off:off + d], both[:, off + d:off + 2 * d].sigmoid()
+            wide = torch.zeros(b, 2 * d + 9, device=dev, dtype=torch.bfloat16)
+            wide[:, off + 1:off + 1 + d] = g
+            s1, slots = torch.randn(b + 5, d, device=dev), torch.randperm(b + 5, device=dev)[:b].contiguous()
+            s2 = s1.clone()
+            assert torch.equal(ops.gated_step(s1, slots, wide[:, off + 1:off + 1 + d], x), ops.gated_step(s2, slots, g.contiguous(), x.contiguous())) and torch.equal(s1, s2)
+
+
 def test_scan_on_other_streams(dev):
     from tensoflow_amd import ops
     ln = [4000, 7, 900]
