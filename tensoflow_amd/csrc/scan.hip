@@ -147,7 +147,8 @@ using namespace tfscan;
 
 namespace {
 
-// A workgroup is a row and 256 V of its channels.  The first row of a slot takes the later ones of the same slot along, in order; the others leave.
+// A workgroup is a row and 256 V of its channels.  Bound: the launch for a few rows (one of 2048 channels 2.3 us), then the states, read and written
+// (256 x 4096 bf16 with 32 fp32 gates: 4.8 us, 2.6 TB/s).  The first row of a slot takes the later ones of the same slot along, in order; the others leave.
 template <typename XT, typename GT, int V, bool SHARED>
 __global__ void __launch_bounds__(256) step_kernel(TfGatedScan d, const GT* __restrict__ gate, const XT* __restrict__ x, const ll* __restrict__ slots,
                                                    ll n_slots, float* __restrict__ state, XT* __restrict__ y) {

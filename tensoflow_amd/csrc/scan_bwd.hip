@@ -9,7 +9,6 @@ using namespace tfscan;
 
 namespace {
 
-
 // sums over the LP lanes of a head of K values: the first lane has them all
 template <int K>
 __device__ __forceinline__ void head_sums(float (&s)[K], int wl, int LP) {
@@ -40,7 +39,10 @@ __device__ __forceinline__ float head_sums_pow2(float (&s)[K], int wl, int LP) {
   return v;
 }
 
-// Packed 16-bit values leave room for two workgroups on a CU (16385 x 2048 bf16 with 16 gates: 119 -> 88 us); fp32 ones do not, and are not squeezed.
+// Registers: 16-bit values stay packed, which leaves room for two workgroups of eight waves on a CU (16385 x 2048 bf16 with 16 gates: 80 us, 119 with x and
+// gy widened and one workgroup); fp32 takes 150 to 230, and three workgroups of four waves or one.  The bound of 2 waves is no squeeze and has to stay
+// one: held to 128 registers, the kernel of 4 x 16-bit channels spilled 63 and one of its four channels came out with wrong states.
+// Measured: 40001 x 512 fp32, a gate for each channel, 101 us (491 MB of which 328 here: 4.1 TB/s of its own reads and writes).
 template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
 __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const float* __restrict__ carry, const XT* __restrict__ gy, const float* __restrict__ gfinal,
                                                        GT* __restrict__ dgate, float* __restrict__ dgate_parts, XT* __restrict__ dx, float* __restrict__ dh0) {

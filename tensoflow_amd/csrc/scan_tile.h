@@ -368,7 +368,7 @@ __device__ __forceinline__ void cut_at(const ScanArgs& p, int k, unsigned cut, u
 }
 
 // The same for all rows of a lane at once, where lanes have rows of their own: row after row, each with a wait for its index and one for its state,
-// the edges of short segments cost more than the rest (8000003 x 4 fp32, 23 rows a segment: 160 us).  Lanes without an edge read a place that is there.
+// the edges of short segments cost more than the rest (8000003 x 4 fp32, 23 rows a segment: 160 us, 123 with all at once).  Lanes without an edge read a place that is there.
 template <bool WIDE>
 __device__ __forceinline__ void segs_of(const ScanArgs& p, const Rows<WIDE>& r, unsigned edge, int (&seg)[K]) {
   ll v[K];
