@@ -12,7 +12,6 @@ typedef unsigned long long ull;
 // Up to SMALL segments every workgroup sums the lengths by itself and finds its rows' segments in LDS: ONE launch, where the sums' own would cost
 // as much again (1024 segments, 130003 rows: 9.6 us of kernels in two, 7.7 in one).  More segments: sums, offsets, rows.
 constexpr int SMALL = 2048;
-constexpr int CHUNK = 2048;  // lengths of a workgroup of the sums
 constexpr int WAVE_ROWS = 1024;  // rows of a wave of the rows
 
 __device__ __forceinline__ ll seg_len(const ll* __restrict__ lengths, ll s, ll n_rows) { return min(max(lengths[s], 0ll), n_rows); }
@@ -117,14 +116,17 @@ __global__ void __launch_bounds__(256) seg_small_kernel(const ll* __restrict__ l
   }
 }
 
-// sums of CHUNK lengths (and of their block counts); the start bits cleared
+// PER lengths a thread: 2 up to a million segments (640000: sums and offsets 20 us, 27 with 8), 16 beyond, where every workgroup adds up the sums of
+// all before it.
+// sums of a workgroup's lengths (and of their block counts); the start bits cleared
+template <int PER>
 __global__ void __launch_bounds__(256) seg_sums_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, Blocks b, ll* __restrict__ sums,
                                                        ull* __restrict__ starts, ll n_words) {
   __shared__ ll part[4];
-  const ll s0 = (ll)blockIdx.x * CHUNK;
+  const ll s0 = (ll)blockIdx.x * (256 * PER);
   ll sum = 0, bsum = 0, total;
 #pragma unroll
-  for (int k = 0; k < CHUNK / 256; ++k) {
+  for (int k = 0; k < PER; ++k) {
     const ll s = s0 + k * 256 + threadIdx.x;
     if (s < n_seg) {
       const ll v = seg_len(lengths, s, n_rows);
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(256) seg_sums_kernel(const ll* __restrict__ le
 }
 
 // offsets from the sums; every segment with rows marks its first one: the start bit, and its number in index
+template <int PER>
 __global__ void __launch_bounds__(256) seg_offsets_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, Blocks b, const ll* __restrict__ sums,
                                                           ll* __restrict__ offsets, ll* __restrict__ block_first, ll* __restrict__ index, ull* __restrict__ starts) {
   __shared__ ll part[4];
@@ -153,11 +156,10 @@ __global__ void __launch_bounds__(256) seg_offsets_kernel(const ll* __restrict__
   base = total;
   block_exclusive<4>(bbase, part, total);
   bbase = total;
-  constexpr int PER = CHUNK / 256;
   ll v[PER], sum = 0, bsum = 0;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const ll s = (ll)blockIdx.x * CHUNK + threadIdx.x * PER + k;
+    const ll s = ((ll)blockIdx.x * 256 + threadIdx.x) * PER + k;
     v[k] = s < n_seg ? seg_len(lengths, s, n_rows) : 0;
     sum += v[k];
     if (b.rows) bsum += blocks_of(b, v[k]);
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(256) seg_offsets_kernel(const ll* __restrict__
   if (b.rows) bbase += block_exclusive<4>(bsum, part, total);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const ll s = (ll)blockIdx.x * CHUNK + threadIdx.x * PER + k, at = min(base, n_rows);
+    const ll s = ((ll)blockIdx.x * 256 + threadIdx.x) * PER + k, at = min(base, n_rows);
     if (s < n_seg) {
       offsets[s] = at;
       if (b.rows) block_first[s] = bbase;
@@ -281,7 +283,8 @@ __global__ void __launch_bounds__(256) seg_starts_kernel(const ll* __restrict__ 
 }
 
 inline bool grid_fits(ll n, ll per) { return (n + per - 1) / per < (1ll << 31); }
-inline ll chunks_of(ll n_seg) { return (n_seg + CHUNK - 1) / CHUNK; }
+inline int per_of(ll n_seg) { return n_seg <= (1 << 20) ? 2 : 16; }
+inline ll chunks_of(ll n_seg) { return (n_seg + 256 * per_of(n_seg) - 1) / (256 * per_of(n_seg)); }
 
 }  // namespace
 
@@ -325,8 +328,16 @@ extern "C" int tf_segment_tables(const int64_t* lengths, int64_t n_segments, int
     ll* first = sums + 2 * chunks_of(n_segments);
     const unsigned grid = (unsigned)chunks_of(n_segments);
     const bool pair = (((size_t)index | (size_t)position | (size_t)slots) & 15) == 0;
-    seg_sums_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ull*)starts, starts ? (n_rows + 63) >> 6 : 0);
-    seg_offsets_kernel<<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ll*)offsets, first, (ll*)index, (ull*)starts);
+    const ll words = starts ? (n_rows + 63) >> 6 : 0;
+#define SUMS(PER)                                                                                                                            \
+  seg_sums_kernel<PER><<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ull*)starts, words);                           \
+  seg_offsets_kernel<PER><<<grid, 256, 0, st>>>((const ll*)lengths, n_segments, n_rows, b, sums, (ll*)offsets, first, (ll*)index, (ull*)starts)
+    if (per_of(n_segments) == 2) {
+      SUMS(2);
+    } else {
+      SUMS(16);
+    }
+#undef SUMS
     if (cells) seg_blocks_kernel<<<(unsigned)((cells + 255) / 256), 256, 0, st>>>((const ll*)lengths, first, n_segments, n_rows, b);
     if (n_rows > 0 && (index || position))
       seg_rows_kernel<<<(unsigned)((n_rows + 4 * WAVE_ROWS - 1) / (4 * WAVE_ROWS)), 256, 0, st>>>((const ll*)offsets, first, n_segments, n_rows, (const ull*)starts,

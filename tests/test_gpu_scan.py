@@ -97,7 +97,7 @@ def test_blocks(dev, block, n_free, width):
     assert np.array_equal(t.block_table.cpu().numpy(), want[4]) and np.array_equal(t.slots.cpu().numpy(), want[5])
 
 
-@pytest.mark.parametrize("r,n", [(1023, 5000), (1024, 3), (4097, 100000), (70001, 200000), (300000, 250)])
+@pytest.mark.parametrize("r,n", [(1023, 5000), (1024, 3), (4097, 100000), (70001, 200000), (300000, 250), (1100000, 3000001)])
 def test_tables_of_many(dev, r, n):
     """Against torch on the host: longer lists than the step-by-step form is made for, runs of a hundred thousand empty segments among them."""
     from tensoflow_amd import ops
