@@ -242,7 +242,9 @@ typedef struct TfGatedScan {
  * offsets / index / starts: of tf_segment_tables or tf_segment_from_index (index is read with h0 or final alone).  carry: NULL, or
  * tf_gated_scan_carry_floats(d) floats that the backward pass needs.
  * tf_gated_scan_bwd: gy [n_rows, channels] (x's type) and gfinal [n_segments, channels], either NULL; dgate [n_rows, gates], dx [n_rows, channels],
- * dh0 [n_segments, channels], each NULL where it is not wanted.  No atomics on results: they repeat bit by bit. */
+ * dh0 [n_segments, channels], each NULL where it is not wanted.  No atomics on results: they repeat bit by bit.
+ * What is not finite in one segment does not reach another.  Within one, |a| <= 1 is meant: a decay, or a product of decays, that is infinite, and an
+ * infinite state whose later decays' product underflows, may give NaN where a step-by-step evaluation gives inf. */
 size_t tf_gated_scan_carry_floats(const TfGatedScan* d);
 size_t tf_gated_scan_workspace_floats(const TfGatedScan* d, int32_t backward);
 int tf_gated_scan_fwd(const TfGatedScan* d, const void* gate, const void* x, const int64_t* offsets, const int64_t* index, const uint64_t* starts,

@@ -1,5 +1,5 @@
 """Packed sequences in 64 bits, step by step: segment tables, the gated linear recurrence with its gradients, its one-token form, and worst-case
-bounds of an fp32 evaluation of it (checker of tf_segment_tables, tf_gated_scan_* and tf_gated_step)."""
+bounds of an fp32 evaluation of it (the oracle of tf_segment_tables, tf_gated_scan_* and tf_gated_step)."""
 import numpy as np
 
 
