@@ -74,9 +74,10 @@ __global__ void __launch_bounds__(512, SHARED || (WIDE && sizeof(XT) == 2) ? 4 :
       for (int v = 0; v < AV; ++v) a[v] = fmaf(a[v], s1, s0);
     }
   };
-  // the states that segments begin from, for all of a lane's rows at once: b + a h0 in the place of b
+  // the states that segments begin from, for all of a lane's rows at once: b + a h0 in the place of b, which is then the first row's state
+  constexpr bool JOINED = !WIDE && WHOLE;
   const float* h0 = p.h0;
-  if (!WIDE && WHOLE && h0) {
+  if (JOINED && h0) {
     if (__any(first)) {
       int seg[K];
       float s[K][V];
@@ -88,7 +89,6 @@ __global__ void __launch_bounds__(512, SHARED || (WIDE && sizeof(XT) == 2) ? 4 :
         for (int v = 0; v < V; ++v)
           x[k].w[v] = __builtin_bit_cast(unsigned, seg[k] >= 0 ? fmaf(g[k][AV == 1 ? 0 : v], s[k][v], x[k][v]) : x[k][v]);
     }
-    h0 = nullptr;
   }
   // a first row begins from h0 (or 0), a row of no segment from 0: it holds b = 0 and leaves 0
   unsigned cut = first | (~r.valid & ((1u << K) - 1));
@@ -100,11 +100,11 @@ __global__ void __launch_bounds__(512, SHARED || (WIDE && sizeof(XT) == 2) ? 4 :
   for (int v = 0; v < V; ++v) B[v] = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    cut_at<V, WIDE>(p, k, cut, first, h0, r.p0 + k * r.step, l.c, B);
+    if (!JOINED) cut_at<V, WIDE>(p, k, cut, first, h0, r.p0 + k * r.step, l.c, B);
     float a[AV], b[V];
     terms(k, a, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) B[v] = fmaf(a[AV == 1 ? 0 : v], B[v], b[v]);
+    for (int v = 0; v < V; ++v) B[v] = JOINED && (cut >> k & 1) ? b[v] : fmaf(a[AV == 1 ? 0 : v], B[v], b[v]);
 #pragma unroll
     for (int v = 0; v < AV; ++v) A[v] *= a[v];
   }
@@ -140,11 +140,11 @@ __global__ void __launch_bounds__(512, SHARED || (WIDE && sizeof(XT) == 2) ? 4 :
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const ll at = r.p0 + k * r.step;
-    cut_at<V, WIDE>(p, k, cut, first, h0, at, l.c, h);
+    if (!JOINED) cut_at<V, WIDE>(p, k, cut, first, h0, at, l.c, h);
     float a[AV], b[V];
     terms(k, a, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = fmaf(a[AV == 1 ? 0 : v], h[v], b[v]);
+    for (int v = 0; v < V; ++v) h[v] = JOINED && (cut >> k & 1) ? b[v] : fmaf(a[AV == 1 ? 0 : v], h[v], b[v]);
     if (l.ok) {
       if (turned) ty.put(buf, p.D, block, l.c, p.reverse, k, round_v<XT, V>(h));
       else if (full || (r.valid >> k & 1) || (p.zero_rest && (r.in >> k & 1))) store_v<XT, V>((y + at * p.D) + l.c, h);

@@ -253,6 +253,19 @@ def test_scan_does_not_cross_segments(dev):
             assert not bool(torch.isfinite(final[1]).any())
 
 
+def test_scan_first_step_with_an_infinite_decay(dev):
+    """a h0 + b at a segment's first row as the formula has it, for short rows and long ones."""
+    from tensoflow_amd import ops
+    for d, g in ((4, 1), (40, 40), (256, 2)):
+        ln = [20, 30, 41]
+        gate, x = inputs(91, d, g, "f32", "f32", "decay", 3)
+        h0 = torch.ones(3, d)
+        gate[20] = float("inf")
+        h0[1, 0] = -1.0
+        y, _ = ops.gated_scan(gate.to(dev), x.to(dev), ops.segment_tables(torch.tensor(ln, device=dev), 91), h0.to(dev))
+        assert bool(torch.isinf(y[20]).all()) and float(y[20, 0]) < 0 < float(y[20, 1]) and bool(torch.isfinite(y[:20]).all()) and bool(torch.isfinite(y[50:]).all())
+
+
 def test_scan_leaves_the_rest(dev):
     from tensoflow_amd import ops
     ln, n, d = [5, 0, 60], 200, 12
