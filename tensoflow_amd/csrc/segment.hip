@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(256) seg_small_kernel(const ll* __restrict__ l
 
 // PER lengths a thread: 2 up to a million segments (640000: sums and offsets 20 us, 27 with 8), 16 beyond, where every workgroup adds up the sums of
 // all before it.
-// sums of a workgroup's lengths (and of their block counts); the start bits cleared
+// sums of a workgroup's lengths (and of their block counts); the start bits cleared.  A sum counts for no more than all rows (all free blocks): what lies
+// behind is cut at the same place, and 2^31 segments of up to 2^39 rows sum to 2^58 at most.
 template <int PER>
 __global__ void __launch_bounds__(256) seg_sums_kernel(const ll* __restrict__ lengths, ll n_seg, ll n_rows, Blocks b, ll* __restrict__ sums,
                                                        ull* __restrict__ starts, ll n_words) {
@@ -135,9 +136,9 @@ __global__ void __launch_bounds__(256) seg_sums_kernel(const ll* __restrict__ le
     }
   }
   block_exclusive<4>(sum, part, total);
-  if (threadIdx.x == 0) sums[2 * blockIdx.x] = total;
+  if (threadIdx.x == 0) sums[2 * blockIdx.x] = min(total, n_rows);
   if (b.rows) block_exclusive<4>(bsum, part, total);
-  if (threadIdx.x == 0) sums[2 * blockIdx.x + 1] = b.rows ? total : 0;
+  if (threadIdx.x == 0) sums[2 * blockIdx.x + 1] = b.rows ? min(total, b.n_free) : 0;
   if (starts)
     for (ll w = (ll)blockIdx.x * 256 + threadIdx.x; w < n_words; w += (ll)gridDim.x * 256) starts[w] = 0;
 }

@@ -1,0 +1,38 @@
+"""Packed sequences: what the documentation of the operators allows and promises at their edges (shapes of gradients, second derivatives, first steps,
+tensors changed between the passes, sums beyond 64 bits)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import recurrence as rec
+from test_gpu_scan import d64, inputs, near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU test collected but no GPU is visible")
+    return torch.device("cuda:0")
+
+
+def test_sums_beyond_64_bits(dev):
+    """Lengths whose plain sum leaves 63 bits are cut like any others."""
+    from tensoflow_amd import ops
+    most, r = 1 << 38, (1 << 25) + 4099
+    off = ops.segment_offsets(torch.full((r,), 1 << 62, dtype=torch.int64, device=dev))
+    assert int(off[0]) == 0 and bool((off[1:] == most).all())
+
+
+def test_block_counts_beyond_64_bits(dev):
+    import ctypes as C
+    from tensoflow_amd import lib as L
+    most, r = 1 << 38, (1 << 25) + 4099
+    lib, new = L.load(), lambda k, t=torch.int64: torch.full((k,), 5, dtype=t, device=dev)
+    lens, off, table, free = new(r).fill_(1 << 62), new(r + 1), new(2 * r, torch.int32), torch.arange(3, dtype=torch.int32, device=dev)
+    nw = lib.tf_segment_workspace_words(r, 1)
+    work = new(nw)
+    L.check(lib.tf_segment_tables(lens.data_ptr(), r, most, off.data_ptr(), None, None, None, 1, free.data_ptr(), 3, 2, table.data_ptr(), None, work.data_ptr(), nw,
+                                  C.c_void_p(torch.cuda.current_stream().cuda_stream)), "tf_segment_tables")
+    assert int(off[0]) == 0 and bool((off[1:] == most).all()) and table[:4].tolist() == [0, 1, -1, -1] and bool((table[2:] == -1).all())
