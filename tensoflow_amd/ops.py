@@ -698,7 +698,8 @@ def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final
 
 
 def gated_scan_bwd(gate, x, tables, carry, gy, g_final, h0=None, form="decay", reverse=False, need_gate=True, need_x=True, need_h0=True):
-    """Gradients of `gated_scan` -> (g_gate, g_x, g_h0) (None where not needed); carry: what the forward pass kept; gy like x and g_final [R, C] may be None."""
+    """Gradients of `gated_scan` -> (g_gate, g_x, g_h0), each of its input's shape (None where not needed); carry: what the forward pass kept; gy like x
+    and g_final [R, C] may be None."""
     stream = _on(x, gate, h0, carry, gy, g_final, tables.offsets)
     R = tables.n_segments
     d, n, c = _scan_desc(gate, x, R, form, reverse, 1)
@@ -715,7 +716,7 @@ def gated_scan_bwd(gate, x, tables, carry, gy, g_final, h0=None, form="decay", r
     pg = C.c_void_p(0) if gy is None else _like_x(gy, x, "gy")
     new = lambda like, ok: torch.empty(like.shape, dtype=like.dtype, device=x.device) if ok else None
     g_gate, g_x = new(gate, need_gate), new(x, need_x)
-    g_h0 = torch.empty(R, *x.shape[1:], dtype=torch.float32, device=x.device) if need_h0 else None
+    g_h0 = torch.empty((R, *x.shape[1:]) if h0 is None else h0.shape, dtype=torch.float32, device=x.device) if need_h0 else None
     nw = lib.tf_gated_scan_workspace_floats(C.byref(d), 1)
     work = torch.empty(nw, dtype=torch.float32, device=x.device) if nw else None
     L.check(lib.tf_gated_scan_bwd(C.byref(d), gate.data_ptr(), x.data_ptr(), tables.offsets.data_ptr(), _p(tables.index, torch.int64), tables.starts.data_ptr(),

@@ -36,3 +36,27 @@ def test_block_counts_beyond_64_bits(dev):
     L.check(lib.tf_segment_tables(lens.data_ptr(), r, most, off.data_ptr(), None, None, None, 1, free.data_ptr(), 3, 2, table.data_ptr(), None, work.data_ptr(), nw,
                                   C.c_void_p(torch.cuda.current_stream().cuda_stream)), "tf_segment_tables")
     assert int(off[0]) == 0 and bool((off[1:] == most).all()) and table[:4].tolist() == [0, 1, -1, -1] and bool((table[2:] == -1).all())
+
+
+@pytest.mark.parametrize("flat", [True, False])
+def test_heads_with_a_start_state(dev, flat):
+    """x [N, H, P] with h0 [R, C] or [R, H, P]: each gradient in its input's shape."""
+    from tensoflow_amd import autograd, ops
+    ln, h, p = [30, 0, 41], 4, 5
+    n = sum(ln)
+    gate, x = inputs(n, h * p, h, "f32", "f32", "decay", 3)
+    r = torch.Generator().manual_seed(1)
+    h0, gy, gf = torch.randn(3, h * p, generator=r), torch.randn(n, h * p, generator=r), torch.randn(3, h * p, generator=r)
+    want = rec.scan(d64(gate), d64(x), rec.tables(ln, n)[0], d64(h0), "decay", False, d64(gy), d64(gf))
+    leaves = [t.to(dev).requires_grad_() for t in (gate, x.view(n, h, p), h0 if flat else h0.view(3, h, p))]
+    tab = ops.segment_tables(torch.tensor(ln, device=dev), n)
+    y, final = autograd.gated_scan(leaves[0], leaves[1], tab, leaves[2])
+    assert y.shape == (n, h, p) and final.shape == (3, h, p)
+    got = torch.autograd.grad((y, final), leaves, (gy.to(dev).view(n, h, p), gf.to(dev).view(3, h, p)))
+    for g, leaf, k in zip(got, leaves, ("g_gate", "g_x", "g_h0")):
+        assert g.shape == leaf.shape
+        near(g, want[k], want[k + "_tol"], k)
+    _, _, carry = ops.gated_scan(leaves[0].detach(), leaves[1].detach(), tab, leaves[2].detach(), want_carry=True)
+    gh = ops.gated_scan_bwd(leaves[0].detach(), leaves[1].detach(), tab, carry, None, gf.to(dev), leaves[2].detach())[2]
+    assert gh.shape == leaves[2].shape
+    assert ops.gated_scan_bwd(leaves[0].detach(), leaves[1].detach(), tab, carry, None, gf.to(dev))[2].shape == (3, h, p)
