@@ -412,6 +412,19 @@ class CompositeFn(torch.autograd.Function):
         return ga, (gvs[0] if len(gvs) == 1 else torch.cat(gvs, -1)), None, None
 
 
+class _OnceFn(torch.autograd.Function):
+    """Hands the gradients t[n:] on unchanged.  t[:n] is what they were computed from: whoever differentiates them with respect to it meets an error instead of
+    a derivative that is silently missing."""
+
+    @staticmethod
+    def forward(ctx, n, *t):
+        return t[n:]
+
+    @staticmethod
+    def backward(ctx, *g):
+        raise RuntimeError("the gated recurrence can be differentiated once: its gradients have no derivative")
+
+
 class GatedScanFn(torch.autograd.Function):
     """(y, final) = the gated linear recurrence over a packed batch (tf_gated_scan_fwd); backward tf_gated_scan_bwd wrt gate, x and h0.  The
     states are computed again in the backward pass, from x and the fp32 states kept every few rows: y may be rounded, its gradient is not."""
@@ -433,11 +446,13 @@ class GatedScanFn(torch.autograd.Function):
         c = lambda t: None if t is None else t.contiguous()
         need = ctx.needs_input_grad
         g = ops.gated_scan_bwd(gate, x, tables, carry, c(gy), c(g_final), h0, form, reverse, need[0], need[1], need[2])
+        if torch.is_grad_enabled():                                                   # create_graph
+            g = _OnceFn.apply(5, gate, x, h0, gy, g_final, *g)
         return (*g, None, None, None)
 
 
 def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False):
-    """Differentiable `ops.gated_scan` -> (y, final) (final None where the tables have no index).  Leaves that a captured graph and eager code
+    """Differentiable (once) `ops.gated_scan` -> (y, final) (final None where the tables have no index).  Leaves that a captured graph and eager code
     both use: take their gradients by torch.autograd.grad, not by accumulation into .grad."""
     rows = lambda t: t if t.dim() < 2 or t[:1].is_contiguous() else t.contiguous()      # channels side by side; any row stride
     return GatedScanFn.apply(rows(gate), rows(x), None if h0 is None else h0.contiguous(), tables, form, reverse)

@@ -60,3 +60,28 @@ def test_heads_with_a_start_state(dev, flat):
     gh = ops.gated_scan_bwd(leaves[0].detach(), leaves[1].detach(), tab, carry, None, gf.to(dev), leaves[2].detach())[2]
     assert gh.shape == leaves[2].shape
     assert ops.gated_scan_bwd(leaves[0].detach(), leaves[1].detach(), tab, carry, None, gf.to(dev))[2].shape == (3, h, p)
+
+
+def test_second_derivative_is_refused(dev):
+    """A gradient taken with create_graph is the same; what depends on it through the recurrence raises, it is not left out of a sum."""
+    from tensoflow_amd import autograd, ops
+    tab = ops.segment_tables(torch.tensor([20, 3], device=dev))
+    for k in range(3):
+        leaves = [torch.rand(23, 2, device=dev), torch.randn(23, 4, device=dev), torch.randn(2, 4, device=dev)]
+        leaves[k].requires_grad_()
+        y, final = autograd.gated_scan(leaves[0], leaves[1], tab, leaves[2])
+        plain, = torch.autograd.grad(y.sum() + final.sum(), leaves[k], retain_graph=True)
+        g, = torch.autograd.grad(y.sum() + final.sum(), leaves[k], create_graph=True)
+        assert torch.equal(g, plain) and g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            ((g ** 2).sum() + (leaves[k] ** 2).sum()).backward()
+    weight = torch.rand(23, 4, device=dev, requires_grad=True)                       # a gradient with respect to what comes from behind
+    x = torch.randn(23, 4, device=dev, requires_grad=True)
+    y, _ = autograd.gated_scan(torch.rand(23, 2, device=dev), x, tab)
+    g, = torch.autograd.grad((y * weight).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(g.sum(), weight)
+    loss = (autograd.gated_scan(torch.rand(23, 2, device=dev), x, tab)[0]).sum() + (weight ** 3).sum()
+    gw, gx = torch.autograd.grad(loss, (weight, x), create_graph=True)                # and where nothing asks for it, nothing is refused
+    gw.sum().backward()
+    assert torch.allclose(weight.grad, 6 * weight) and gx.shape == x.shape
