@@ -432,15 +432,16 @@ class GatedScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, tables, form, reverse):
         y, final, carry = ops.gated_scan(gate, x, tables, h0, form, reverse, want_final=tables.index is not None, want_carry=True)
-        ctx.save_for_backward(gate, x, h0, carry)
-        ctx.cfg = (tables, form, reverse)
+        ctx.save_for_backward(gate, x, h0, carry, tables.offsets, tables.index, tables.starts)
+        ctx.cfg = (tables.n_rows, tables.n_segments, form, reverse)
         ctx.set_materialize_grads(False)
         return y, final
 
     @staticmethod
     def backward(ctx, gy, g_final):
-        gate, x, h0, carry = ctx.saved_tensors
-        tables, form, reverse = ctx.cfg
+        gate, x, h0, carry, offsets, index, starts = ctx.saved_tensors
+        n_rows, n_segments, form, reverse = ctx.cfg
+        tables = ops.SegmentTables(n_rows, n_segments, offsets, index, None, starts)
         if gy is None and g_final is None:
             return None, None, None, None, None, None
         c = lambda t: None if t is None else t.contiguous()

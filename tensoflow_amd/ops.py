@@ -692,8 +692,11 @@ def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final
     work = new(nw)
     L.check(lib.tf_gated_scan_fwd(C.byref(d), gate.data_ptr(), x.data_ptr(), tables.offsets.data_ptr(), _p(tables.index, torch.int64), tables.starts.data_ptr(),
                                   ph, py, _p(final), _p(carry), _p(work), nw, stream), "tf_gated_scan_fwd")
-    if out is not None and y is not out:
-        y = out.copy_(y)
+    if out is not None:
+        if y is not out:
+            y = out.copy_(y)
+        else:
+            torch.autograd.graph.increment_version(out)                               # written behind torch's back: a graph that saved it sees the change
     return (y, final, carry) if want_carry else (y, final)
 
 
@@ -742,6 +745,7 @@ def gated_step(state, slots, gate, x, form="decay", out=None):
         return y
     L.check(L.load().tf_gated_step(C.byref(d), gate.data_ptr(), x.data_ptr(), _p(slots, torch.int64, "slots"), state.shape[0],
                                    _p(state, torch.float32, "state"), _like_x(y, x, "out"), stream), "tf_gated_step")
+    torch.autograd.graph.increment_version(state if out is None else (state, out))    # written behind torch's back: a graph that saved them sees the change
     return y
 
 

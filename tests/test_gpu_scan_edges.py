@@ -85,3 +85,39 @@ def test_second_derivative_is_refused(dev):
     gw, gx = torch.autograd.grad(loss, (weight, x), create_graph=True)                # and where nothing asks for it, nothing is refused
     gw.sum().backward()
     assert torch.allclose(weight.grad, 6 * weight) and gx.shape == x.shape
+
+
+def test_changes_between_the_passes_are_seen(dev):
+    """A pool stepped in place, an `out` and the tables count as changed: a backward pass that needs what they held raises."""
+    from tensoflow_amd import autograd, ops
+    changed = "modified by an inplace operation"
+    lens = torch.tensor([20, 3], device=dev)
+    gate, x, pool = torch.rand(23, 2, device=dev), torch.randn(23, 4, device=dev), torch.randn(2, 4, device=dev)
+
+    def forward():
+        tab = ops.segment_tables(lens)
+        leaf, data = gate.clone().requires_grad_(), x.clone()
+        return tab, leaf, data, autograd.gated_scan(leaf, data, tab, pool)[0].sum()
+    tab, leaf, data, loss = forward()
+    torch.autograd.grad(loss, leaf)
+    _, leaf, _, loss = forward()
+    ops.gated_step(pool, torch.tensor([1], device=dev), gate[:1], x[:1])
+    with pytest.raises(RuntimeError, match=changed):
+        torch.autograd.grad(loss, leaf)
+    tab, leaf, data, loss = forward()
+    ops.gated_scan(gate, x, tab, out=data)
+    with pytest.raises(RuntimeError, match=changed):
+        torch.autograd.grad(loss, leaf)
+    _, leaf, data, loss = forward()
+    ops.gated_step(pool.clone(), torch.tensor([1], device=dev), gate[:1], x[:1], out=data[2:3])
+    with pytest.raises(RuntimeError, match=changed):
+        torch.autograd.grad(loss, leaf)
+    for name in ("offsets", "index", "starts"):
+        tab, leaf, _, loss = forward()
+        getattr(tab, name).add_(0)
+        with pytest.raises(RuntimeError, match=changed):
+            torch.autograd.grad(loss, leaf)
+    with torch.inference_mode():                                                      # tensors without a count of their changes
+        state = torch.zeros(2, 4, device=dev)
+        ops.gated_step(state, torch.tensor([1, 0], device=dev), gate[:2], x[:2])
+        ops.gated_scan(gate, x, ops.segment_tables(lens), out=torch.empty(23, 4, device=dev))
