@@ -74,21 +74,26 @@ __global__ void __launch_bounds__(512, SHARED || (WIDE && sizeof(XT) == 2) ? 4 :
       for (int v = 0; v < AV; ++v) a[v] = fmaf(a[v], s1, s0);
     }
   };
-  // the states that segments begin from, for all of a lane's rows at once: b + a h0 in the place of b, which is then the first row's state
+  // the states that segments begin from (0 where there is no h0), for all of a lane's rows at once: b + a h0 in the place of b, which is then the first row's
+  // state.  The product with a 0 stays: an infinite decay gives here what it gives in the other kernels and in the backward pass.
   constexpr bool JOINED = !WIDE && WHOLE;
   const float* h0 = p.h0;
-  if (JOINED && h0) {
-    if (__any(first)) {
+  if (JOINED && __any(first)) {
+    float s[K][V] = {};
+    if (h0) {
       int seg[K];
-      float s[K][V];
       segs_of<WIDE>(p, r, first, seg);
       states_of<V>(p, h0, seg, l.c, s);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-          x[k].w[v] = __builtin_bit_cast(unsigned, seg[k] >= 0 ? fmaf(g[k][AV == 1 ? 0 : v], s[k][v], x[k][v]) : x[k][v]);
+        for (int v = 0; v < V; ++v) s[k][v] = seg[k] >= 0 ? s[k][v] : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        x[k].w[v] = __builtin_bit_cast(unsigned, first >> k & 1 ? fmaf(g[k][AV == 1 ? 0 : v], s[k][v], x[k][v]) : x[k][v]);
   }
   // a first row begins from h0 (or 0), a row of no segment from 0: it holds b = 0 and leaves 0
   unsigned cut = first | (~r.valid & ((1u << K) - 1));

@@ -121,3 +121,31 @@ def test_changes_between_the_passes_are_seen(dev):
         state = torch.zeros(2, 4, device=dev)
         ops.gated_step(state, torch.tensor([1, 0], device=dev), gate[:2], x[:2])
         ops.gated_scan(gate, x, ops.segment_tables(lens), out=torch.empty(23, 4, device=dev))
+
+
+@pytest.mark.parametrize("t,gt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("d,g", [(4, 1), (10, 1), (12, 12), (40, 40), (40, 10), (256, 2), (260, 260)])
+def test_first_steps_without_a_start_state(dev, d, g, t, gt):
+    """No h0 is an h0 of zeros, also where a first row's decay is infinite or NaN: a 0 + b in every kernel and in both passes."""
+    from tensoflow_amd import ops
+    ln = [20, 30, 41, 9]
+    n = sum(ln)
+    for form in ("decay", "log"):
+        for reverse in (False, True):
+            gate, x = inputs(n, d, g, t, gt, form, d)
+            gy = torch.randn(n, d, generator=torch.Generator().manual_seed(2)).to(x.dtype)
+            first = [19, 49, 90, 99] if reverse else [0, 20, 50, 91]
+            gate[first[1]], gate[first[2]] = float("inf"), float("nan")
+            off = rec.tables(ln, n)[0]
+            with np.errstate(invalid="ignore"):
+                want = rec.scan(d64(gate), d64(x), off, None, form, reverse, d64(gy), None)
+            tab = ops.segment_tables(torch.tensor(ln, device=dev), n)
+            res = []
+            for h0 in (None, torch.zeros(4, d, device=dev)):
+                y, final, carry = ops.gated_scan(gate.to(dev), x.to(dev), tab, h0, form, reverse, want_final=True, want_carry=True)
+                res.append((y, final, *ops.gated_scan_bwd(gate.to(dev), x.to(dev), tab, carry, gy.to(dev), None, h0, form, reverse)))
+            for a, b, k in zip(*res, ("y", "final", "g_gate", "g_x", "g_h0")):
+                assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0)), k
+                fine = np.isfinite(want[k])
+                assert np.array_equal(a.isfinite().cpu().numpy(), fine), (k, form, reverse)
+                near(a[torch.from_numpy(fine).to(dev)], want[k][fine], want[k + "_tol"][fine], k)
