@@ -43,11 +43,9 @@ Geo geometry(const TfGatedScan& d) {
   const int most = d.x_type == TF_TYPE_F32 || D < 64 ? 4 : 8;
   g.nw = most;
   while (g.nw > 1 && ((d.n_rows + g.nw * wave_rows - 1) / (g.nw * wave_rows)) * g.slabs < 512) g.nw >>= 1;
-  for (int w = 1; w <= most; w <<= 1)
-    if (d.n_rows <= w * wave_rows && w > g.nw) {
-      g.nw = w;
-      break;
-    }
+  int all = 1;  // waves that hold all rows, no more than that
+  while (all < most && d.n_rows > all * wave_rows) all <<= 1;
+  if (d.n_rows <= all * wave_rows) g.nw = all;
   g.tile_rows = g.nw * wave_rows;
   g.tiles = (d.n_rows + g.tile_rows - 1) / g.tile_rows;
   return g;
