@@ -441,7 +441,7 @@ class GatedScanFn(torch.autograd.Function):
     def backward(ctx, gy, g_final):
         gate, x, h0, carry, offsets, index, starts = ctx.saved_tensors
         n_rows, n_segments, form, reverse = ctx.cfg
-        tables = ops.SegmentTables(n_rows, n_segments, offsets, index, None, starts)
+        tables = ops.SegmentTables.__new__(ops.SegmentTables)._set(n_rows, n_segments, offsets, index, None, starts)
         if gy is None and g_final is None:
             return None, None, None, None, None, None
         c = lambda t: None if t is None else t.contiguous()

@@ -521,8 +521,17 @@ class SegmentTables:
     __slots__ = ("n_rows", "n_segments", "offsets", "index", "position", "starts", "block_table", "slots")
 
     def __init__(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None):
+        for name, t, n in (("offsets", offsets, n_segments + 1), ("starts", starts, (n_rows + 63) // 64), ("index", index, n_rows)):
+            if t is None and name == "index":
+                continue
+            if t is None or t.dtype != torch.int64 or t.numel() != n or not t.is_contiguous():      # the kernels take these sizes as given
+                raise RuntimeError(f"{name} of {n_rows} rows in {n_segments} segments must be contiguous int64 [{n}]")
+        self._set(n_rows, n_segments, offsets, index, position, starts, block_table, slots)
+
+    def _set(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None):
         self.n_rows, self.n_segments, self.offsets, self.index, self.position = n_rows, n_segments, offsets, index, position
         self.starts, self.block_table, self.slots = starts, block_table, slots
+        return self
 
 
 def _on(*tensors):
@@ -570,7 +579,8 @@ def segment_tables(lengths, n_rows=None, index=True, position=True, block_rows=0
     if n_rows < 0 or block_rows < 0:
         raise RuntimeError("n_rows and block_rows must not be negative")
     new = lambda *s, dtype=torch.int64: torch.empty(s, dtype=dtype, device=dev)
-    t = SegmentTables(n_rows, R, new(R + 1), new(n_rows) if index or block_rows else None, new(n_rows) if position else None, new((n_rows + 63) // 64))
+    t = SegmentTables.__new__(SegmentTables)._set(n_rows, R, new(R + 1), new(n_rows) if index or block_rows else None, new(n_rows) if position else None,
+                                                  new((n_rows + 63) // 64))
     lib, n_free = L.load(), 0
     if block_rows:
         if free_blocks is None:
@@ -595,8 +605,8 @@ def segment_tables_from_index(index, n_segments):
     stream = _on(index)
     pi = _p(index, torch.int64, "index")
     n, dev = index.shape[0], index.device
-    t = SegmentTables(n, n_segments, torch.empty(n_segments + 1, dtype=torch.int64, device=dev), index, None,
-                      torch.empty((n + 63) // 64, dtype=torch.int64, device=dev))
+    t = SegmentTables.__new__(SegmentTables)._set(n, n_segments, torch.empty(n_segments + 1, dtype=torch.int64, device=dev), index, None,
+                                                  torch.empty((n + 63) // 64, dtype=torch.int64, device=dev))
     L.check(L.load().tf_segment_from_index(pi, n, n_segments, t.offsets.data_ptr(), t.starts.data_ptr(), stream), "tf_segment_from_index")
     return t
 
