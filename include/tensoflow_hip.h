@@ -238,7 +238,8 @@ typedef struct TfGatedScan {
 } TfGatedScan;
 
 /* y [n_rows, channels] (x's type) = h of every row that is a segment's; final [n_segments, channels] or NULL:
- * the state after the segment's last step, h0 (or 0) where it has no rows; h0 [n_segments, channels] or NULL.
+ * the state after the segment's last step, h0 (or 0) where it has no rows; h0 [n_segments, channels], or NULL for zeros (a first row is a h0 + b in
+ * either case, so its infinite or NaN decay gives NaN there).
  * offsets / index / starts: of tf_segment_tables or tf_segment_from_index (index is read with h0 or final alone).  carry: NULL, or
  * tf_gated_scan_carry_floats(d) floats that the backward pass needs.
  * tf_gated_scan_bwd: gy [n_rows, channels] (x's type) and gfinal [n_segments, channels], either NULL; dgate [n_rows, gates], dx [n_rows, channels],

@@ -38,8 +38,8 @@ Geo geometry(const TfGatedScan& d) {
   g.W = g.CL * g.V;
   const ll wave_rows = (64 / g.CL) * K;
   // waves of a workgroup: as many as leave two workgroups to every CU, or as hold all rows in one tile
-  // (four at most where rows are shorter than a cache line: their buffers take 9 KB of LDS a wave; and for fp32, whose kernels' registers leave room
-  // for 12 waves on a CU: three workgroups of four, where eight waves would be alone)
+  // (four at most where rows are shorter than a cache line: their buffers take 9 KB of LDS a wave; and for fp32, most of whose kernels' registers leave
+  // room for 12 waves on a CU: three workgroups of four, where eight waves would be alone)
   const int most = d.x_type == TF_TYPE_F32 || D < 64 ? 4 : 8;
   g.nw = most;
   while (g.nw > 1 && ((d.n_rows + g.nw * wave_rows - 1) / (g.nw * wave_rows)) * g.slabs < 512) g.nw >>= 1;

@@ -39,10 +39,13 @@ __device__ __forceinline__ float head_sums_pow2(float (&s)[K], int wl, int LP) {
   return v;
 }
 
-// Registers: 16-bit values stay packed, which leaves room for two workgroups of eight waves on a CU (16385 x 2048 bf16 with 16 gates: 80 us, 119 with x and
-// gy widened and one workgroup); fp32 takes 150 to 230, and three workgroups of four waves or one.  The bound of 2 waves is no squeeze and has to stay
-// one: held to 128 registers, the kernel of 4 x 16-bit channels spilled 63 and one of its four channels came out with wrong states.
-// Measured: 40001 x 512 fp32, a gate for each channel, 101 us (491 MB of which 328 here: 4.1 TB/s of its own reads and writes).
+// Registers: 16-bit values stay packed.  With shared gates and a wave across the channels that takes 98 to 115 vector registers, two workgroups of eight waves
+// on a CU (16385 x 2048 bf16 with 16 gates: 81 us, 119 with x and gy widened and one workgroup).  The other kernels of four 16-bit channels take 135 to
+// 172: one workgroup of eight waves, or two to three of four (rows under 64 channels).  fp32 takes 94 to 167, three workgroups of four waves or more; its
+// narrow kernels of three and four channels a lane 176 to 230, two of them.  The bound of 2 waves squeezes none of them and has to stay so:
+// held to 128 registers, a kernel of 4 x 16-bit channels spilled 63 and one of its four channels came out with wrong states.  No mistake was found in
+// the source, so no_spills.py ends the build of such a kernel.  Scalar registers are spilled in all of them, 102 to 181, into lanes of vector registers.
+// Measured: 40001 x 512 fp32, a gate for each channel, 102 us (491 MB of which 328 here: 4.1 TB/s of its own reads and writes).
 template <typename XT, typename GT, int V, bool SHARED, bool WIDE>
 __global__ void __launch_bounds__(512, 2) scan_bwd_kernel(ScanArgs p, const float* __restrict__ carry, const XT* __restrict__ gy, const float* __restrict__ gfinal,
                                                        GT* __restrict__ dgate, float* __restrict__ dgate_parts, XT* __restrict__ dx, float* __restrict__ dh0) {

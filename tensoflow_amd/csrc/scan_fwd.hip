@@ -6,8 +6,9 @@ using namespace tfscan;
 
 namespace {
 
-// No kernel here may spill registers (the bounds below are the tightest that none does).  Measured: 65536 x 1024 bf16 with a bf16 gate for each channel, one
-// sequence, 131 us (403 MB, 3.1 TB/s): a tile of 15 us spends 4.6 on its loads, 1.5 on its own map, 5.8 on its place in the chain and 2.5 on its stores, and two
+// No kernel here may spill vector registers (no_spills.py ends the build; the bounds below are the tightest that none does).  Scalar registers are spilled in
+// all of them, 75 to 106, into lanes of vector registers.  Measured: 65536 x 1024 bf16 with a bf16 gate for each channel, one sequence, 134 us (403 MB, 3.0
+// TB/s): a tile of 15 us spends 4.6 on its loads, 1.5 on its own map, 5.8 on its place in the chain and 2.5 on its stores, and two
 // tiles to a CU do not fill each other's pauses.  Tried and slower: 16 rows a lane (155 us, registers), 4 rows (180), workgroups that stay and touch their next
 // tile's lines ahead (161), the next tile's rows held in registers (they spill).
 template <typename XT, typename GT, int V, bool SHARED, bool WIDE>

@@ -199,7 +199,7 @@ __device__ __forceinline__ ll wave_seg_of(const ll* __restrict__ offsets, ll n_s
 }
 
 // Every row from the start bits: a row belongs to the last start at or before it, among the wave's 128 rows or carried from before.  A lane has two rows
-// side by side, stored as one piece of 16 bytes (33.3 million rows, 640000 segments, two tables: 153 us with a row and 8 bytes a lane).
+// side by side, stored as one piece of 16 bytes (33.3 million rows, 640000 segments, two tables: 91 us; 180 with a row and 8 bytes a lane).
 typedef ll ll2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void put2(ll* p, ll i, ll n, bool pair, ll a, ll b) {
   if (pair && i + 1 < n) {

@@ -551,7 +551,7 @@ _MOST_ROWS = 1 << 38
 
 
 def segment_offsets(lengths):
-    """Exclusive sums [R + 1] of the int64 lengths [R] of a packed batch (the first table of `segment_tables` alone; offsets[-1] rows in all)."""
+    """Exclusive sums [R + 1] of the int64 lengths [R] of a packed batch (the first table of `segment_tables` alone; offsets[-1] rows in all, 2^38 at most)."""
     if lengths.dim() != 1:
         raise RuntimeError(f"lengths must be [R], got {tuple(lengths.shape)}")
     stream = _on(lengths)
@@ -568,7 +568,7 @@ def segment_tables(lengths, n_rows=None, index=True, position=True, block_rows=0
     """SegmentTables of the int64 lengths [R] of a packed batch.  n_rows: the number of rows (of the packed tensors); None: the lengths' sum, with one
     host read.  Rows behind the last segment get index and position -1; lengths that sum to more are cut there.
     block_rows > 0: also block_table [R, max_blocks] int32 and slots [N] of rows kept in blocks of a shared store, the blocks dealt in order from
-    free_blocks (int32; None: 0, 1, 2 ...); max_blocks: width of the table (None: as many as n_rows could need)."""
+    free_blocks (int32; None: 0, 1, 2 ...); max_blocks: width of the table (None: as many as one segment of all n_rows needs; name it where R is large)."""
     if lengths.dim() != 1:
         raise RuntimeError(f"lengths must be [R], got {tuple(lengths.shape)}")
     stream = _on(lengths, free_blocks)
@@ -678,7 +678,7 @@ def _state(t, n, c, name):
 def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final=False, out=None, want_carry=False):
     """h_t = a_t h_{t-1} + b_t along every segment of `tables` -> (y, final): y like x holds every h_t, final [R, C] fp32 the last ones (None unless
     wanted).  form "decay": a = gate, b = x; "log": a = exp(gate), b = x; "alpha": a = 1 - gate, b = gate x.  x [N, C] (or [N, H, P]) fp32 / fp16 / bf16;
-    gate [N], [N, G] or like x, of x's type or fp32, each serving C / G consecutive channels.  h0 [R, C] fp32: the states before the first step.  reverse: from
+    gate [N], [N, G] or like x, of x's type or fp32, each serving C / G consecutive channels.  h0 [R, C] fp32: the states before the first step (None: 0).  reverse: from
     each segment's last row to its first.  out: written in x's place of y, rows of no segment left as they are (without it they are 0).
     want_carry: -> (y, final, carry) for `gated_scan_bwd`."""
     stream = _on(x, gate, h0, out, tables.offsets)
