@@ -432,24 +432,28 @@ class GatedScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, tables, form, reverse):
         y, final, carry = ops.gated_scan(gate, x, tables, h0, form, reverse, want_final=tables.index is not None, want_carry=True)
-        ctx.save_for_backward(gate, x, h0, carry, tables.offsets, tables.index, tables.starts)
-        ctx.cfg = (tables.n_rows, tables.n_segments, form, reverse)
+        # h0's values enter the gate's gradient alone
+        ctx.save_for_backward(gate, x, h0 if ctx.needs_input_grad[0] else None, carry, tables.offsets, tables.index, tables.starts)
+        ctx.cfg = (tables.n_rows, tables.n_segments, form, reverse, None if h0 is None else h0.shape)
         ctx.set_materialize_grads(False)
         return y, final
 
     @staticmethod
     def backward(ctx, gy, g_final):
         gate, x, h0, carry, offsets, index, starts = ctx.saved_tensors
-        n_rows, n_segments, form, reverse = ctx.cfg
+        n_rows, n_segments, form, reverse, h0_shape = ctx.cfg
         tables = ops.SegmentTables.__new__(ops.SegmentTables)._set(n_rows, n_segments, offsets, index, None, starts)
         if gy is None and g_final is None:
             return None, None, None, None, None, None
         c = lambda t: None if t is None else t.contiguous()
         need = ctx.needs_input_grad
-        g = ops.gated_scan_bwd(gate, x, tables, carry, c(gy), c(g_final), h0, form, reverse, need[0], need[1], need[2])
-        if torch.is_grad_enabled():                                                   # create_graph
-            g = _OnceFn.apply(5, gate, x, h0, gy, g_final, *g)
-        return (*g, None, None, None)
+        g_gate, g_x, g_h0 = ops.gated_scan_bwd(gate, x, tables, carry, c(gy), c(g_final), h0, form, reverse, need[0], need[1], need[2])
+        if g_h0 is not None:
+            g_h0 = g_h0.view(h0_shape)
+        if torch.is_grad_enabled():                                                   # create_graph; y is linear in x and h0, their gradients do not depend on them
+            g_gate, = _OnceFn.apply(5, gate, x, h0, gy, g_final, g_gate)
+            g_x, g_h0 = _OnceFn.apply(3, gate, gy, g_final, g_x, g_h0)
+        return g_gate, g_x, g_h0, None, None, None
 
 
 def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False):

@@ -72,9 +72,21 @@ def test_second_derivative_is_refused(dev):
         y, final = autograd.gated_scan(leaves[0], leaves[1], tab, leaves[2])
         plain, = torch.autograd.grad(y.sum() + final.sum(), leaves[k], retain_graph=True)
         g, = torch.autograd.grad(y.sum() + final.sum(), leaves[k], create_graph=True)
-        assert torch.equal(g, plain) and g.requires_grad
+        assert torch.equal(g, plain) and g.requires_grad == (k == 0)
+        loss = (g ** 2).sum() + (leaves[k] ** 2).sum()
+        if k == 0:
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                loss.backward()
+        else:                                                                         # y is linear in x and h0: that part of the derivative is 0
+            loss.backward()
+            assert torch.equal(leaves[k].grad, 2 * leaves[k].detach())
+    leaves = [torch.rand(23, 2, device=dev, requires_grad=True), torch.randn(23, 4, device=dev, requires_grad=True), torch.randn(2, 4, device=dev, requires_grad=True)]
+    y, final = autograd.gated_scan(leaves[0], leaves[1], tab, leaves[2])
+    grads = torch.autograd.grad(y.sum() + final.sum(), leaves, create_graph=True)
+    for a, b in ((0, 0), (0, 1), (0, 2), (1, 0), (2, 0)):                             # the gate's gradient depends on all three, the others on the gate
         with pytest.raises(RuntimeError, match="differentiated once"):
-            ((g ** 2).sum() + (leaves[k] ** 2).sum()).backward()
+            torch.autograd.grad(grads[a].sum(), leaves[b], retain_graph=True)
+    assert torch.autograd.grad(grads[1].sum() + leaves[1].sum(), leaves[1])[0].eq(1).all()
     weight = torch.rand(23, 4, device=dev, requires_grad=True)                       # a gradient with respect to what comes from behind
     x = torch.randn(23, 4, device=dev, requires_grad=True)
     y, _ = autograd.gated_scan(torch.rand(23, 2, device=dev), x, tab)
@@ -117,6 +129,11 @@ def test_changes_between_the_passes_are_seen(dev):
         getattr(tab, name).add_(0)
         with pytest.raises(RuntimeError, match=changed):
             torch.autograd.grad(loss, leaf)
+    data = x.clone().requires_grad_()                                                 # x's gradient does not depend on the start state
+    want, = torch.autograd.grad(autograd.gated_scan(gate, data, tab, pool)[0].sum(), data)
+    loss = autograd.gated_scan(gate, data, tab, pool)[0].sum()
+    ops.gated_step(pool, torch.tensor([1], device=dev), gate[:1], x[:1])
+    assert torch.equal(torch.autograd.grad(loss, data)[0], want)
     with torch.inference_mode():                                                      # tensors without a count of their changes
         state = torch.zeros(2, 4, device=dev)
         ops.gated_step(state, torch.tensor([1, 0], device=dev), gate[:2], x[:2])
