@@ -442,13 +442,13 @@ class GatedScanFn(torch.autograd.Function):
     def backward(ctx, gy, g_final):
         gate, x, h0, carry, offsets, index, starts = ctx.saved_tensors
         n_rows, n_segments, form, reverse, h0_shape = ctx.cfg
-        tables = ops.SegmentTables.__new__(ops.SegmentTables)._set(n_rows, n_segments, offsets, index, None, starts)
+        tables = ops.SegmentTables(n_rows, n_segments, offsets, index, None, starts, _built=True)
         if gy is None and g_final is None:
             return None, None, None, None, None, None
         c = lambda t: None if t is None else t.contiguous()
         need = ctx.needs_input_grad
         g_gate, g_x, g_h0 = ops.gated_scan_bwd(gate, x, tables, carry, c(gy), c(g_final), h0, form, reverse, need[0], need[1], need[2])
-        if g_h0 is not None:
+        if h0 is None and g_h0 is not None:                                           # h0 was not saved
             g_h0 = g_h0.view(h0_shape)
         if torch.is_grad_enabled():                                                   # create_graph; y is linear in x and h0, their gradients do not depend on them
             g_gate, = _OnceFn.apply(5, gate, x, h0, gy, g_final, g_gate)

@@ -520,18 +520,16 @@ class SegmentTables:
     starts [ceil(N / 64)] (one bit a row), block_table [R, M] and slots [N]; what was not asked for is None."""
     __slots__ = ("n_rows", "n_segments", "offsets", "index", "position", "starts", "block_table", "slots")
 
-    def __init__(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None):
+    def __init__(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None, _built=False):
+        self.n_rows, self.n_segments, self.offsets, self.index, self.position = n_rows, n_segments, offsets, index, position
+        self.starts, self.block_table, self.slots = starts, block_table, slots
+        if _built:
+            return
         for name, t, n in (("offsets", offsets, n_segments + 1), ("starts", starts, (n_rows + 63) // 64), ("index", index, n_rows)):
             if t is None and name == "index":
                 continue
             if t is None or t.dtype != torch.int64 or t.numel() != n or not t.is_contiguous():      # the kernels take these sizes as given
                 raise RuntimeError(f"{name} of {n_rows} rows in {n_segments} segments must be contiguous int64 [{n}]")
-        self._set(n_rows, n_segments, offsets, index, position, starts, block_table, slots)
-
-    def _set(self, n_rows, n_segments, offsets, index, position, starts, block_table=None, slots=None):
-        self.n_rows, self.n_segments, self.offsets, self.index, self.position = n_rows, n_segments, offsets, index, position
-        self.starts, self.block_table, self.slots = starts, block_table, slots
-        return self
 
 
 def _on(*tensors):
@@ -548,6 +546,7 @@ def _on(*tensors):
 
 
 _MOST_ROWS = 1 << 38
+_written = torch.autograd.graph.increment_version       # of a tensor that a kernel wrote behind torch's back: a graph that saved it sees the change
 
 
 def segment_offsets(lengths):
@@ -579,8 +578,7 @@ def segment_tables(lengths, n_rows=None, index=True, position=True, block_rows=0
     if n_rows < 0 or block_rows < 0:
         raise RuntimeError("n_rows and block_rows must not be negative")
     new = lambda *s, dtype=torch.int64: torch.empty(s, dtype=dtype, device=dev)
-    t = SegmentTables.__new__(SegmentTables)._set(n_rows, R, new(R + 1), new(n_rows) if index or block_rows else None, new(n_rows) if position else None,
-                                                  new((n_rows + 63) // 64))
+    t = SegmentTables(n_rows, R, new(R + 1), new(n_rows) if index or block_rows else None, new(n_rows) if position else None, new((n_rows + 63) // 64), _built=True)
     lib, n_free = L.load(), 0
     if block_rows:
         if free_blocks is None:
@@ -605,8 +603,8 @@ def segment_tables_from_index(index, n_segments):
     stream = _on(index)
     pi = _p(index, torch.int64, "index")
     n, dev = index.shape[0], index.device
-    t = SegmentTables.__new__(SegmentTables)._set(n, n_segments, torch.empty(n_segments + 1, dtype=torch.int64, device=dev), index, None,
-                                                  torch.empty((n + 63) // 64, dtype=torch.int64, device=dev))
+    t = SegmentTables(n, n_segments, torch.empty(n_segments + 1, dtype=torch.int64, device=dev), index, None,
+                      torch.empty((n + 63) // 64, dtype=torch.int64, device=dev), _built=True)
     L.check(L.load().tf_segment_from_index(pi, n, n_segments, t.offsets.data_ptr(), t.starts.data_ptr(), stream), "tf_segment_from_index")
     return t
 
@@ -706,7 +704,7 @@ def gated_scan(gate, x, tables, h0=None, form="decay", reverse=False, want_final
         if y is not out:
             y = out.copy_(y)
         else:
-            torch.autograd.graph.increment_version(out)                               # written behind torch's back: a graph that saved it sees the change
+            _written(out)
     return (y, final, carry) if want_carry else (y, final)
 
 
@@ -755,7 +753,9 @@ def gated_step(state, slots, gate, x, form="decay", out=None):
         return y
     L.check(L.load().tf_gated_step(C.byref(d), gate.data_ptr(), x.data_ptr(), _p(slots, torch.int64, "slots"), state.shape[0],
                                    _p(state, torch.float32, "state"), _like_x(y, x, "out"), stream), "tf_gated_step")
-    torch.autograd.graph.increment_version(state if out is None else (state, out))    # written behind torch's back: a graph that saved them sees the change
+    _written(state)
+    if out is not None:
+        _written(out)
     return y
 
 
